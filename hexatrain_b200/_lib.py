@@ -29,6 +29,9 @@ HX_ATTN_CUDA_CORES = 1
 HX_OPT_ADAM = 0
 HX_OPT_MUON = 1
 HX_OPT_MOMENTUM = 2
+HX_DTYPE_F32 = 0
+HX_DTYPE_BF16 = 1
+HX_DTYPE_F16 = 2
 HX_STABILITY_LEGACY = 0
 HX_STABILITY_WARMUP64 = 1
 HX_STABILITY_DECAY_LINEAR = 2
@@ -195,6 +198,19 @@ SIGNATURES = {
     "hx_lm_checkpoint_resume": (C.c_int, [C.c_void_p, C.c_char_p, C.c_uint32, C.c_uint32, C.c_char_p,
                                           C.POINTER(NprtInfoC)]),
 }
+
+# The operators on device logits: dtype, rows, vocab, logits, stride, and for
+# distillation the record, the labels, the temperature and the weights.
+_ROWS = [C.c_void_p, C.c_int, C.c_uint32, C.c_uint32, C.c_void_p, C.c_size_t]
+_DISTILL = _ROWS + [C.c_uint32] + [C.c_void_p] * 4 + [C.c_float] * 3
+SIGNATURES.update({
+    "hx_top_logits_device": (C.c_int, _ROWS + [C.c_uint32, C.c_float] + [C.c_void_p] * 3),
+    "hx_distill_forward_device": (C.c_int, _DISTILL + [C.c_void_p] * 2),
+    "hx_distill_backward_device": (C.c_int, _DISTILL + [C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_size_t]),
+    "hx_distill_forward_backward_device": (C.c_int, _DISTILL + [C.c_void_p, C.c_float, C.c_void_p, C.c_void_p,
+                                                                C.c_size_t]),
+    "hx_sample_logits_device": (C.c_int, _ROWS + [C.c_void_p] * 7),
+})
 
 _LIB = None
 

@@ -145,6 +145,9 @@ struct Profiler {
 // 11-14, the Muon kernel 16, and the wait self-test
 // (hx_runtime_check_wait_timeout).
 constexpr int kWaitProbeCode = 21;
+// Error-word code of the kernels over logit rows: a teacher index or a label
+// that is not below the vocabulary size.
+constexpr int kHeadIndexCode = 31;
 
 struct MlpPlan;
 struct LmPlan;
@@ -217,6 +220,9 @@ struct hx_runtime {
         if (code) {
             hx::check_cuda(cudaMemsetAsync(err_flag.ptr, 0, sizeof(int), stream), "cudaMemsetAsync");
             hx::check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
+            if (code == hx::kHeadIndexCode)
+                hx::fail(HX_ERR_ARGUMENT, "INVALID_DISTILL_INDEX: a teacher index or label is not below the vocabulary "
+                                          "size; results of this call are invalid");
             const char* where = code >= hx::kWaitProbeCode ? "wait self-test"
                                 : code >= 16               ? "tensor-core Muon"
                                 : code >= 10               ? "tensor-core attention"

@@ -702,3 +702,54 @@ class Runtime:
             self._rt, rows, cols, ptr(w), ptr(_f32(gradient)), ptr(_f32(momentum_buffer)), learning_rate, momentum,
             int(nesterov), ns_steps, abc[0], abc[1], abc[2], int(bf16_inputs), ptr(wn), ptr(bn)))
         return ok, wn, bn
+
+    # -- operators on device logits ------------------------------------------------
+    # Pointers are integers (e.g. torch.Tensor.data_ptr()), 0 for an absent
+    # one; dtype is _lib.HX_DTYPE_F32 / _BF16 / _F16; row r of the logits starts
+    # at logits + r * stride elements.  All run on the runtime's stream without
+    # synchronising (set_stream: 1 names the legacy default stream).
+    def top_logits_device(self, dtype: int, rows: int, vocab: int, logits: int, stride: int, k: int, values: int,
+                          indices: int, lse: int = 0, temperature: float = 1.0) -> bool:
+        """The k largest logits of every row in order, and the row's log-sum-exp
+        at `temperature` where lse is given (hx_top_logits_device)."""
+        return self._need() and self._ok(self._lib.hx_top_logits_device(
+            self._rt, dtype, rows, vocab, logits, stride, k, temperature, values, indices, lse))
+
+    def distill_forward_device(self, dtype: int, rows: int, vocab: int, logits: int, stride: int, k: int,
+                               teacher_values: int, teacher_indices: int, teacher_lse: int, labels: int,
+                               temperature: float, kd_weight: float, ce_weight: float, loss: int, stats: int) -> bool:
+        """Per-row distillation loss and the statistics [rows, 3] its backward
+        reads (hx_distill_forward_device)."""
+        return self._need() and self._ok(self._lib.hx_distill_forward_device(
+            self._rt, dtype, rows, vocab, logits, stride, k, teacher_values, teacher_indices, teacher_lse, labels,
+            temperature, kd_weight, ce_weight, loss, stats))
+
+    def distill_backward_device(self, dtype: int, rows: int, vocab: int, logits: int, stride: int, k: int,
+                                teacher_values: int, teacher_indices: int, teacher_lse: int, labels: int,
+                                temperature: float, kd_weight: float, ce_weight: float, stats: int, d_logits: int,
+                                grad_stride: int, grad_loss: int = 0, grad_scale: float = 1.0) -> bool:
+        """The gradient of the distillation loss from its statistics, times
+        grad_scale and grad_loss[row] (hx_distill_backward_device)."""
+        return self._need() and self._ok(self._lib.hx_distill_backward_device(
+            self._rt, dtype, rows, vocab, logits, stride, k, teacher_values, teacher_indices, teacher_lse, labels,
+            temperature, kd_weight, ce_weight, stats, grad_loss, grad_scale, d_logits, grad_stride))
+
+    def distill_forward_backward_device(self, dtype: int, rows: int, vocab: int, logits: int, stride: int, k: int,
+                                        teacher_values: int, teacher_indices: int, teacher_lse: int, labels: int,
+                                        temperature: float, kd_weight: float, ce_weight: float, loss: int,
+                                        d_logits: int, grad_stride: int, grad_loss: int = 0,
+                                        grad_scale: float = 1.0) -> bool:
+        """Loss and gradient in one pass over the logits; d_logits may be the
+        logits themselves (hx_distill_forward_backward_device)."""
+        return self._need() and self._ok(self._lib.hx_distill_forward_backward_device(
+            self._rt, dtype, rows, vocab, logits, stride, k, teacher_values, teacher_indices, teacher_lse, labels,
+            temperature, kd_weight, ce_weight, grad_loss, grad_scale, loss, d_logits, grad_stride))
+
+    def sample_logits_device(self, dtype: int, rows: int, vocab: int, logits: int, stride: int, uniform: int,
+                             tokens: int, log_probs: int = 0, temperature: int = 0, top_k: int = 0, top_p: int = 0,
+                             min_p: int = 0) -> bool:
+        """One token for every row from uniform[rows], with per-row settings in
+        device arrays (hx_sample_logits_device)."""
+        return self._need() and self._ok(self._lib.hx_sample_logits_device(
+            self._rt, dtype, rows, vocab, logits, stride, uniform, temperature, top_k, top_p, min_p, tokens,
+            log_probs))

@@ -516,6 +516,75 @@ int hx_lm_checkpoint_save(hx_runtime* rt, const char* path, uint32_t seed, uint3
 int hx_lm_checkpoint_resume(hx_runtime* rt, const char* path, uint32_t expected_seed,
                             uint32_t expected_step, const char* tokenizer_hash, hx_nprt_info* info);
 
+/* ---- operators on device logits ------------------------------------------ */
+/* Top logits, distillation and sampling over rows of logits [rows, vocab] in
+ * device memory: row r starts at logits + r * stride elements (stride >=
+ * vocab, any alignment of the type), vocab <= 262144.  No prepare is needed and
+ * nothing is allocated after a runtime's first call.  The calls are
+ * asynchronous on the runtime's stream and must not overlap their outputs with
+ * their inputs except where stated.  rows = 0 does nothing. */
+enum { HX_DTYPE_F32 = 0, HX_DTYPE_BF16 = 1, HX_DTYPE_F16 = 2 };
+
+/* The k largest logits of every row, value descending, the lowest index first
+ * among equals (a NaN ranks after -inf): values[rows*k] in float32,
+ * indices[rows*k], and, where lse is not NULL, lse[rows] = log sum_i
+ * exp(l_i / temperature), the normaliser of the record's tail.  1 <= k <=
+ * min(256, vocab). */
+int hx_top_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,
+                         size_t stride, uint32_t k, float temperature, float* values, int32_t* indices,
+                         float* lse);
+
+/* Distillation from a teacher's top logits.  With tau = temperature,
+ * p = softmax(l / tau) and the teacher's entries (t_j, i_j), j < k <= 256:
+ *   teacher_lse NULL: q = softmax_j(t_j / tau) over the entries;
+ *   otherwise q_j = exp(t_j / tau - teacher_lse[row]) and the rest of the
+ *   teacher's mass, q_T = max(0, 1 - sum_j q_j), is one bucket against the
+ *   student's mass p_T outside the record;
+ *   KL = sum_j q_j (log q_j - log p_{i_j}) [+ q_T (log q_T - log p_T)],
+ *   loss[row] = kd_weight tau^2 KL + ce_weight (logsumexp(l) - l_label).
+ * An entry with i_j < 0 is empty; the entries of one row name distinct tokens.
+ * A row without entries (or, renormalised, with none above -inf) has no KL
+ * term; one whose label is negative, or every row when labels is NULL, has no
+ * hard term; with neither, loss and gradient are 0.  Where the record leaves
+ * the student no mass (p_T = 0) the tail bucket is left out.  An index or label
+ * not below vocab is skipped, and the next synchronising call fails with
+ * "INVALID_DISTILL_INDEX: ...".
+ *
+ * _forward writes loss[rows] and stats[rows*3] = (logsumexp(l/tau),
+ * logsumexp(l), q_T/p_T), which _backward reads; _forward_backward does both in
+ * one pass over the logits.  The gradient, in the type of the logits, is
+ * grad_scale * grad_loss[row] (1 where grad_loss is NULL) * dloss/dl;
+ * d_logits may be the logits themselves (with the same stride). */
+int hx_distill_forward_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,
+                              size_t stride, uint32_t k, const float* teacher_values,
+                              const int32_t* teacher_indices, const float* teacher_lse, const int32_t* labels,
+                              float temperature, float kd_weight, float ce_weight, float* loss, float* stats);
+int hx_distill_backward_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,
+                               size_t stride, uint32_t k, const float* teacher_values,
+                               const int32_t* teacher_indices, const float* teacher_lse, const int32_t* labels,
+                               float temperature, float kd_weight, float ce_weight, const float* stats,
+                               const float* grad_loss, float grad_scale, void* d_logits, size_t grad_stride);
+int hx_distill_forward_backward_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab,
+                                       const void* logits, size_t stride, uint32_t k, const float* teacher_values,
+                                       const int32_t* teacher_indices, const float* teacher_lse,
+                                       const int32_t* labels, float temperature, float kd_weight, float ce_weight,
+                                       const float* grad_loss, float grad_scale, float* loss, void* d_logits,
+                                       size_t grad_stride);
+
+/* One token for every row from uniform[rows] in [0, 1), with per-row settings
+ * in device memory (NULL: off): temperature (NULL: 1; <= 0 or not finite: the
+ * first largest logit), top_k (<= 0: the whole vocabulary), then top_p (>= 1:
+ * off) of what top-k keeps, and min_p (<= 0: off) against the most likely
+ * token.  The order and the walk along the cumulative mass are those of
+ * hx_sample_next_token, with masses in whole numbers (floor(2^31 exp((l -
+ * max)/T))), so the same inputs give the same tokens on every call.
+ * log_probs[rows] (may be NULL): the token's log-probability among the kept
+ * ones.  A row of -inf only gives token -1 and -inf, a row with NaN or +inf
+ * token -1 and NaN. */
+int hx_sample_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,
+                            size_t stride, const float* uniform, const float* temperature, const int32_t* top_k,
+                            const float* top_p, const float* min_p, int32_t* tokens, float* log_probs);
+
 #ifdef __cplusplus
 }
 #endif
