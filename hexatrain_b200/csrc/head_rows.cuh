@@ -41,6 +41,7 @@ __device__ __forceinline__ float from_descending_key(uint32_t k) {
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
 
 struct SumOp {
     template <class T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
@@ -56,6 +57,13 @@ __device__ __forceinline__ T warp_reduce(T v, Op op) {
     return v;
 }
 
+// The largest of the warp's values (not NaN).
+__device__ __forceinline__ float warp_max(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // Reduction over the block's NT threads; every thread gets the result.
 // `scratch` holds NT / 32 values and may be reused after the call returns.
 template <int NT, class T, class Op>
@@ -68,6 +76,285 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, Op op) {
     for (int w = 1; w < NT / 32; ++w) r = op(r, scratch[w]);
     __syncthreads();
     return r;
+}
+
+// ---- a row held in registers -------------------------------------------------
+// A team of NT threads holds up to 32 NT logits of one row (or of one slice of
+// it: the CTAs of a cluster each hold one), 32 to a thread, so that the row is
+// read from memory once.  The row is seen as 16-byte chunks that are aligned
+// in memory; the first chunk begins `lead` elements before the row, and chunk
+// c holds elements [c EPV - lead, c EPV - lead + EPV).  Thread t holds chunks
+// first + t + j NT, so a warp reads 512 consecutive bytes and the index order
+// is (j, t, element).  Chunks at the ends are read and written by element.
+constexpr int kPerThread = 32;
+
+template <class T>
+struct Chunk {
+    static constexpr int EPV = 16 / int(sizeof(T));   // elements of a 16-byte chunk
+    static constexpr int N = kPerThread / EPV;         // chunks of a thread
+    static __device__ __forceinline__ void unpack(const uint4& raw, float (&x)[EPV]);
+    static __device__ __forceinline__ uint4 pack(const float (&x)[EPV]);
+};
+template <>
+__device__ __forceinline__ void Chunk<float>::unpack(const uint4& raw, float (&x)[4]) {
+    x[0] = __uint_as_float(raw.x);
+    x[1] = __uint_as_float(raw.y);
+    x[2] = __uint_as_float(raw.z);
+    x[3] = __uint_as_float(raw.w);
+}
+template <>
+__device__ __forceinline__ uint4 Chunk<float>::pack(const float (&x)[4]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+template <>
+__device__ __forceinline__ void Chunk<__nv_bfloat16>::unpack(const uint4& raw, float (&x)[8]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // a bfloat16 is the upper half of a float32
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+template <>
+__device__ __forceinline__ uint4 Chunk<__nv_bfloat16>::pack(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <>
+__device__ __forceinline__ void Chunk<__half>::unpack(const uint4& raw, float (&x)[8]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ uint4 Chunk<__half>::pack(const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 b = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Where a team's slice of a row lies.  Whole chunks take the unrolled path; the
+// chunk that begins before the row and the one that ends after it are handled
+// by their one thread, element by element.
+template <class T, int NT>
+struct Slice {
+    static constexpr int EPV = Chunk<T>::EPV, N = Chunk<T>::N;
+    int vocab, lead, first, last, thread;  // chunks [first, last)
+    int mine, w0, w1;                      // this thread's first chunk; whole chunks [w0, w1) of the slice
+    bool aligned;                          // chunks are aligned in memory
+    __device__ __forceinline__ Slice(const T* row, int vocab_, int thread_, int rank, int slices)
+        : vocab(vocab_), lead(int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))), thread(thread_), aligned(true) {
+        int chunks = (vocab + lead + EPV - 1) / EPV;
+        if (chunks > slices * NT * N) {  // the lead would not fit (kMaxVocab logits, not aligned): by element
+            lead = 0;
+            aligned = false;
+            chunks = (vocab + EPV - 1) / EPV;
+        }
+        const int each = (chunks + slices - 1) / slices;
+        first = min(chunks, rank * each);
+        last = min(chunks, first + each);
+        mine = first + thread;
+        w0 = max(first, lead > 0 ? 1 : 0);
+        w1 = min(last, (vocab + lead) / EPV);
+    }
+    __device__ __forceinline__ int index(int j, int r) const { return (mine + j * NT) * EPV + r - lead; }
+    __device__ __forceinline__ bool holds(int i) const { return i + lead >= first * EPV && i + lead < last * EPV; }
+    __device__ __forceinline__ bool whole(int j) const { return mine + j * NT >= w0 && mine + j * NT < w1; }
+    // The partial chunks of the slice: -1 where there is none.
+    __device__ __forceinline__ int head() const { return first == 0 && w0 == 1 && last > 0 ? 0 : -1; }
+    __device__ __forceinline__ int tail() const {
+        const int c = (vocab + lead) / EPV;
+        return c >= max(first, w0) && c < last && (vocab + lead) % EPV != 0 ? c : -1;
+    }
+
+    // issues the loads of the whole chunks
+    __device__ __forceinline__ void fetch(const T* row, uint4 (&raw)[N]) const {
+        if (!aligned) return;
+        const uint4* p = reinterpret_cast<const uint4*>(row - lead) + mine;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (whole(j)) raw[j] = p[j * NT];
+    }
+    // v[j EPV + r] = element index(j, r), -inf where there is none
+    __device__ __forceinline__ void values(const T* row, const uint4 (&raw)[N], float (&v)[kPerThread]) const {
+        if (!aligned) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int r = 0; r < EPV; ++r) {
+                    const int i = index(j, r);
+                    v[j * EPV + r] = mine + j * NT < last && i < vocab ? to_float(row[i]) : -INFINITY;
+                }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float x[EPV];
+            Chunk<T>::unpack(raw[j], x);
+            const bool ok = whole(j);
+#pragma unroll
+            for (int r = 0; r < EPV; ++r) v[j * EPV + r] = ok ? x[r] : -INFINITY;
+        }
+        if (const int c = head(); c == 0 && thread == 0)
+            place(row, c, v);
+        if (const int c = tail(); c >= 0 && (c - mine) % NT == 0)
+            place(row, c, v);
+    }
+    __device__ __forceinline__ void place(const T* row, int c, float (&v)[kPerThread]) const {
+        const int at = (c - mine) / NT;
+        float x[EPV];
+#pragma unroll
+        for (int r = 0; r < EPV; ++r) {
+            const int i = c * EPV + r - lead;
+            x[r] = i >= 0 && i < vocab ? to_float(row[i]) : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int r = 0; r < EPV; ++r)
+                if (j == at) v[j * EPV + r] = x[r];
+    }
+    // writes v to `out`, by chunks where out is aligned as the row is
+    __device__ __forceinline__ void store(T* out, const float (&v)[kPerThread]) const {
+        if (!aligned || int((reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T)) != lead) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int r = 0; r < EPV; ++r) {
+                    const int i = index(j, r);
+                    if (mine + j * NT < last && i >= 0 && i < vocab) out[i] = from_float<T>(v[j * EPV + r]);
+                }
+            return;
+        }
+        uint4* p = reinterpret_cast<uint4*>(out - lead) + mine;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float x[EPV];
+#pragma unroll
+            for (int r = 0; r < EPV; ++r) x[r] = v[j * EPV + r];
+            if (whole(j)) p[j * NT] = Chunk<T>::pack(x);
+        }
+        if (const int c = head(); c == 0 && thread == 0)
+            write(out, c, v);
+        if (const int c = tail(); c >= 0 && (c - mine) % NT == 0)
+            write(out, c, v);
+    }
+    __device__ __forceinline__ void write(T* out, int c, const float (&v)[kPerThread]) const {
+        const int at = (c - mine) / NT;
+#pragma unroll
+        for (int r = 0; r < EPV; ++r) {
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j == at) x = v[j * EPV + r];
+            const int i = c * EPV + r - lead;
+            if (i >= 0 && i < vocab) out[i] = from_float<T>(x);
+        }
+    }
+};
+
+// Split cluster barrier: the first phase shows that every CTA of the cluster
+// has started, so that its shared memory may be written.
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_remote(uint32_t addr, float4 x) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w)
+                 : "memory");
+}
+
+// Launch of `rows` teams of `slices` CTAs each, a cluster per row when there
+// are several (over 8 only for a kernel that is opted in to them).
+template <class... KArgs, class... Args>
+inline void launch_rows(void (*kernel)(KArgs...), unsigned grid, int threads, int slices, bool cluster, size_t smem,
+                        cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster && slices > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = slices;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    cfg.attrs = attr;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    if (e != cudaSuccess) (void)cudaGetLastError();  // reported here, not by the next launch
+    check_cuda(e, "kernel launch");
+}
+
+// Teams of `slices` CTAs (a cluster where there are several) that the GPU holds at
+// once: persistent kernels launch no more, since one that had to wait would
+// take a second round of its own.  Asked once for each shape.
+template <class... KArgs>
+inline int resident_teams(hx_runtime* rt, void (*kernel)(KArgs...), int threads, size_t smem, int slices) {
+    struct Known {
+        const void* kernel;
+        size_t smem;
+        int device, slices, teams;
+    };
+    static thread_local std::vector<Known> known;
+    const void* id = reinterpret_cast<const void*>(kernel);
+    for (const Known& x : known)
+        if (x.kernel == id && x.smem == smem && x.device == rt->device && x.slices == slices) return x.teams;
+    int teams = 0;
+    if (slices == 1) {
+        HX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&teams, kernel, threads, smem));
+        teams *= rt->sm_count;
+    } else {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(slices));
+        cfg.blockDim = dim3(unsigned(threads));
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = unsigned(slices);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        HX_CUDA(cudaOccupancyMaxActiveClusters(&teams, kernel, &cfg));
+    }
+    require(teams >= 1, HX_ERR_UNSUPPORTED, "the device does not hold " + std::to_string(slices) + " blocks of a row");
+    if (known.size() >= 256) known.clear();
+    known.push_back({id, smem, rt->device, slices, teams});
+    return teams;
+}
+
+// The chunks a row can take: the largest lead that any of the rows has.
+inline long row_chunks(const void* logits, size_t stride, uint32_t rows, uint32_t vocab, int elem_bytes) {
+    const int epv = 16 / elem_bytes;
+    const uintptr_t base = reinterpret_cast<uintptr_t>(logits);
+    const bool same = rows <= 1 || stride * elem_bytes % 16 == 0;
+    const long lead = same ? long(base % 16) / elem_bytes : epv - 1;
+    return (long(vocab) + lead + epv - 1) / epv;
+}
+// Slices of a row of `chunks` chunks: as few as hold it, and more, down to
+// `least` chunks each, while the rows alone would leave SMs idle.
+inline int row_slices(uint32_t rows, long chunks, long held, long least, int sm_count) {
+    int s = 1;
+    while (s < 16 && chunks > held * s) s *= 2;
+    while (s < 8 && long(rows) * s * 2 <= sm_count && chunks / (2 * s) >= least) s *= 2;
+    return s;
 }
 
 inline size_t element_bytes(int dtype)

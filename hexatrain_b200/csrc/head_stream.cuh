@@ -1,0 +1,88 @@
+// head_stream.cuh -- rows of logits streamed through shared memory.
+//
+// A persistent block takes row after row (or, in a cluster, its slice of each).
+// One producer warp copies the row's aligned 16-byte chunks with
+// cp.async.bulk into a ring of slots, as far ahead as the ring has room, while the
+// NT consumer threads work: a slot holds NT chunks, thread t reads chunk t of
+// every slot.  The loads of the next rows are in flight through all of a row's
+// reductions and barriers, which is what a memory-bound row operator of short
+// phases needs: with one row per block and loads straight to registers the
+// same arithmetic reached 41-50 % of the bandwidth this form reaches.
+//
+// Every wait is bounded; one that runs out records a code, sets the block's
+// abort flag and lets every other wait pass, so that all loops and barriers run
+// to their end and the block leaves in order.
+#pragma once
+
+#include "head_rows.cuh"
+
+namespace hx {
+namespace head {
+
+struct WaitState {
+    int* err;               // the runtime's error word
+    volatile int* aborted;  // in shared memory
+};
+__device__ __forceinline__ void stream_wait(uint64_t* bar, uint32_t parity, const WaitState& w) {
+    if (tc::mbar_try_wait(bar, parity)) return;
+    const long long t0 = clock64();
+    while (!tc::mbar_try_wait(bar, parity)) {
+        if (*w.aborted) return;
+        if (clock64() - t0 > tc::kWaitCycles) {
+            atomicCAS(w.err, 0, kHeadWaitCode);
+            *w.aborted = 1;
+            return;
+        }
+    }
+}
+
+// Copies `bytes` (a multiple of 16, both ends 16-byte aligned) to this block's
+// shared memory, completing on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     tc::smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+// Stores 16 bytes to a cluster CTA's shared memory, completing on its barrier.
+__device__ __forceinline__ void store_async(uint32_t addr, float4 x, uint32_t bar) {
+    asm volatile(
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "f"(x.x),
+        "f"(x.y), "f"(x.z), "f"(x.w), "r"(bar)
+        : "memory");
+}
+// A place in the ring: slots in turn, the phase changes with every round.
+struct RingCursor {
+    int slot;
+    uint32_t phase;
+    __device__ __forceinline__ void next(int ring) {
+        if (++slot == ring) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// A slice of a row in chunks: chunk c holds elements [c EPV - lead, + EPV).
+template <class T>
+struct Span {
+    static constexpr int EPV = Chunk<T>::EPV;
+    const T* row;
+    int vocab, lead, first, last, w0, w1;  // chunks [first, last), whole ones [w0, w1)
+    __device__ __forceinline__ Span(const T* row_, int vocab_, int rank, int log_slices)
+        : row(row_), vocab(vocab_), lead(int((reinterpret_cast<uintptr_t>(row_) & 15) / sizeof(T))) {
+        const int chunks = (vocab + lead + EPV - 1) / EPV, each = (chunks + (1 << log_slices) - 1) >> log_slices;
+        first = min(chunks, rank * each);
+        last = min(chunks, first + each);
+        w0 = max(first, lead > 0 ? 1 : 0);
+        w1 = max(w0, min(last, (vocab + lead) / EPV));
+    }
+    __device__ __forceinline__ int chunks() const { return last - first; }
+    __device__ __forceinline__ bool holds(int i) const { return i + lead >= first * EPV && i + lead < last * EPV; }
+    // position of element i in the slice
+    __device__ __forceinline__ int position(int i) const { return i + lead - first * EPV; }
+    __device__ __forceinline__ bool whole(int c) const { return c >= w0 && c < w1; }
+};
+
+}  // namespace head
+}  // namespace hx

@@ -142,12 +142,13 @@ struct Profiler {
 };
 
 // Error-word codes of the bounded waits: GEMM roles 1-4, attention roles
-// 11-14, the Muon kernel 16, and the wait self-test
-// (hx_runtime_check_wait_timeout).
+// 11-14, the Muon kernel 16, the wait self-test
+// (hx_runtime_check_wait_timeout) 21, and the kernels over logit rows 32.
 constexpr int kWaitProbeCode = 21;
 // Error-word code of the kernels over logit rows: a teacher index or a label
 // that is not below the vocabulary size.
 constexpr int kHeadIndexCode = 31;
+constexpr int kHeadWaitCode = 32;  // a bounded wait of theirs
 
 struct MlpPlan;
 struct LmPlan;
@@ -223,7 +224,8 @@ struct hx_runtime {
             if (code == hx::kHeadIndexCode)
                 hx::fail(HX_ERR_ARGUMENT, "INVALID_DISTILL_INDEX: a teacher index or label is not below the vocabulary "
                                           "size; results of this call are invalid");
-            const char* where = code >= hx::kWaitProbeCode ? "wait self-test"
+            const char* where = code >= hx::kHeadWaitCode    ? "logit rows"
+                                : code >= hx::kWaitProbeCode ? "wait self-test"
                                 : code >= 16               ? "tensor-core Muon"
                                 : code >= 10               ? "tensor-core attention"
                                                            : "tensor-core GEMM";
