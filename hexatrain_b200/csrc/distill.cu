@@ -418,39 +418,7 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
     if (slices > 1) tc::cluster_sync(); else __syncthreads();
 
     if (warp == NW) {
-        // ---- producer: the slices' chunks into the ring ----
-        RingCursor at{0, 1};  // a fresh barrier lets a wait for phase 1 pass
-        unsigned filled = 0;
-        for (size_t row = team; row < rows; row += teams) {
-            const Span<T> span = span_of(row);
-            // an element of the row's partial chunks: the first (lanes 0-7), the last (8-15)
-            const int r = lane & 7, pc = lane < 8 ? span.first : span.last - 1;
-            const bool partial = lane < 16 && r < EPV && span.chunks() > 0 && !span.whole(pc);
-            const int pi = pc * EPV + r - span.lead;
-            const T px = partial && pi >= 0 && pi < V ? span.row[pi] : from_float<T>(-INFINITY);
-            for (int c0 = span.first; c0 < span.last; c0 += kSlot) {
-                stream_wait(empty + at.slot, at.phase, ws);
-                T* to = reinterpret_cast<T*>(smem) + at.slot * (kSlot * EPV);
-                const int c1 = min(c0 + kSlot, span.last);
-                if (partial && pc >= c0 && pc < c1) {
-                    to[(pc - c0) * EPV + r] = px;
-                    tc::fence_proxy_async_smem();
-                }
-                __syncwarp();
-                if (lane == 0) {
-                    const int b0 = max(c0, span.w0), b1 = min(c1, span.w1);
-                    const uint32_t bytes = b1 > b0 ? uint32_t(b1 - b0) * 16 : 0;
-                    tc::mbar_arrive_expect_tx(full + at.slot, bytes);
-                    if (bytes)
-                        bulk_load(to + (b0 - c0) * EPV, span.row - span.lead + size_t(b0) * EPV, bytes, full + at.slot);
-                }
-                at.next(ring);
-                ++filled;
-            }
-        }
-        if (s_aborted)  // leave with no copy in flight
-            for (unsigned i = filled > unsigned(ring) ? filled - ring : 0; i < filled; ++i)
-                for (int n = 0; n < 1000000 && !tc::mbar_try_wait(full + i % ring, (i / ring) & 1); ++n) {}
+        stream_producer<T, kSlot>(smem, full, empty, ring, rows, team, teams, span_of, ws);
     } else if (warp > NW) {
         // ---- the rows' warps ----
         const int b = warp - NW - 1;

@@ -84,5 +84,46 @@ struct Span {
     __device__ __forceinline__ bool whole(int c) const { return c >= w0 && c < w1; }
 };
 
+// The producer warp: the chunks of rows team, team + teams, ... into the ring's
+// slots of kSlot chunks.
+template <class T, int kSlot, class SpanOf>
+__device__ __forceinline__ void stream_producer(uint8_t* smem, uint64_t* full, uint64_t* empty, int ring, uint32_t rows,
+                                                size_t team, size_t teams, SpanOf span_of, const WaitState& ws) {
+    constexpr int EPV = Chunk<T>::EPV;
+    const int lane = threadIdx.x & 31;
+    RingCursor at{0, 1};  // a fresh barrier lets a wait for phase 1 pass
+    unsigned filled = 0;
+    for (size_t row = team; row < rows; row += teams) {
+        const Span<T> span = span_of(row);
+        // an element of the row's partial chunks: the first (lanes 0-7), the last (8-15)
+        const int r = lane & 7, pc = lane < 8 ? span.first : span.last - 1;
+        const bool partial = lane < 16 && r < EPV && span.chunks() > 0 && !span.whole(pc);
+        const int pi = pc * EPV + r - span.lead;
+        const T px = partial && pi >= 0 && pi < span.vocab ? span.row[pi] : from_float<T>(-INFINITY);
+        for (int c0 = span.first; c0 < span.last; c0 += kSlot) {
+            stream_wait(empty + at.slot, at.phase, ws);
+            T* to = reinterpret_cast<T*>(smem) + at.slot * (kSlot * EPV);
+            const int c1 = min(c0 + kSlot, span.last);
+            if (partial && pc >= c0 && pc < c1) {
+                to[(pc - c0) * EPV + r] = px;
+                tc::fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) {
+                const int b0 = max(c0, span.w0), b1 = min(c1, span.w1);
+                const uint32_t bytes = b1 > b0 ? uint32_t(b1 - b0) * 16 : 0;
+                tc::mbar_arrive_expect_tx(full + at.slot, bytes);
+                if (bytes)
+                    bulk_load(to + (b0 - c0) * EPV, span.row - span.lead + size_t(b0) * EPV, bytes, full + at.slot);
+            }
+            at.next(ring);
+            ++filled;
+        }
+    }
+    if (*ws.aborted)  // leave with no copy in flight
+        for (unsigned i = filled > unsigned(ring) ? filled - ring : 0; i < filled; ++i)
+            for (int n = 0; n < 1000000 && !tc::mbar_try_wait(full + i % ring, (i / ring) & 1); ++n) {}
+}
+
 }  // namespace head
 }  // namespace hx

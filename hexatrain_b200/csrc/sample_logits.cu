@@ -19,7 +19,7 @@
 // -inf gets token -1 and -inf; one with a NaN or +inf gets -1 and NaN.
 //
 // No row is sorted.  y >= 0, so its bits order it: a histogram of counts and
-// masses over the bits (32 buckets to an octave) finds the bucket in which a
+// masses over the bits (64 buckets to an octave) finds the bucket in which a
 // prefix crosses an amount; the bucket's few tokens are collected and sorted.
 #include <cmath>
 
@@ -73,150 +73,248 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t addr, uint32_t x) {
 }
 
 constexpr int kBuckets = 512;
+constexpr uint32_t kHeadKey = 0x41000000u;    // bits of 8.0: the first histogram's end
 constexpr uint32_t kTopKey = 0x42000000u;     // bits of 32.0: above it no token has mass
-constexpr int kFirstShift = 18;               // 32 buckets to an octave
-constexpr int kList = 512;                    // tokens that are collected and sorted at once
+constexpr int kFirstShift = 17;               // 64 buckets to an octave, from 1/32
+constexpr uint32_t kFirstKey = kHeadKey - (uint32_t(kBuckets) << kFirstShift);
+constexpr int kList = 128;                    // tokens that are collected and sorted at once
+constexpr int kPerLane = kBuckets / 32;
 
-// What the cluster's first CTA has the others do.
+// A pass over the row, asked for by the first warp of the first CTA.
 enum SampleStep { kDone = 0, kHistogram, kCollect, kNth };
 struct SampleCommand {
     int step;
-    uint32_t lo, hi;  // keys [lo, hi)
-    int shift;
-    uint32_t nth;     // kNth: which of the tokens with key lo
+    uint32_t lo, hi;    // keys [lo, hi)
+    uint32_t lo2, hi2;  // kCollect: and [lo2, hi2)
+    int shift;          // kHistogram: bucket = (key - lo2) >> shift, 0 below lo2
+    uint32_t nth;       // kNth: which of the tokens with key lo
+    int level, sums;    // kHistogram: where to; with the sums beyond hi
+};
+
+// What the thinking warp keeps between passes.
+enum Goal { kTopK, kTopP, kToken };
+struct Thought {
+    int goal, pending, head_count, refine_shift;  // pending: the step whose result is awaited, -1 at first
+    bool by_count, head, planned;
+    uint64_t W, amount, mass, least, total, plan_mass;
+    uint32_t count, lo, hi, tokens;
+    uint32_t plan_hi;           // the end of the second interval, for the token that follows
 };
 
 struct SampleShared {
     uint32_t low[kBuckets], high[kBuckets], count[kBuckets];  // this slice's: mass = high 2^16 + low
-    uint64_t mass[2][kBuckets];                               // the row's prefix masses before each bucket
-    uint32_t tokens[2][kBuckets];                             // and counts; [0] of the first histogram
-    uint64_t total[2];
+    uint64_t mass[2][kBuckets];                               // the row's, of the first histogram and the last
+    uint32_t tokens[2][kBuckets];
+    uint64_t lane_mass[2][33];                                // before a lane's buckets, and in all
+    uint32_t lane_tokens[2][33];
     uint64_t list[kList];                                     // key 2^32 + index
     uint64_t scan[32];
     float maxima[16];
-    uint64_t min_mass[16];
-    uint32_t nth_counts[16];
-    uint32_t listed, found_bucket;
-    uint64_t found_mass;
-    uint32_t found_count;
+    uint64_t rest_mass[16], min_mass[16];                     // beyond the first histogram; within min-p's limit
+    uint32_t rest_tokens[16], nth_counts[16];
+    uint32_t listed;
     SampleCommand command;
-    int nan;
+    Thought thought;
 };
 
-// Inclusive prefix sums over the block's threads; `total` is the last.
-template <int NT>
-__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* scratch, uint64_t& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The largest element of a chunk, NaN if one is NaN.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float chunk_max(const uint4& raw, float) {
+    return max_or_nan(max_or_nan(__uint_as_float(raw.x), __uint_as_float(raw.y)),
+                      max_or_nan(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+}
+__device__ __forceinline__ float chunk_max(const uint4& raw, __nv_bfloat16) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const __nv_bfloat162 x = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_or_nan(__low2float(x), __high2float(x));
+}
+__device__ __forceinline__ float chunk_max(const uint4& raw, __half) {
+    const __half2* h = reinterpret_cast<const __half2*>(&raw);
+    const __half2 x = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_or_nan(__low2float(x), __high2float(x));
+}
+
+// A warp's prefix sums of 64-bit numbers.
+__device__ __forceinline__ uint64_t warp_scan(uint64_t x) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 31) scratch[warp] = x;
-    __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) before += scratch[w];
-        total += scratch[w];
-    }
-    __syncthreads();
-    return x + before;
+    return x;
 }
 
-// Sorts n <= kList numbers; entries up to the next power of two are written.
-template <int NT>
-__device__ __forceinline__ void block_sort(uint64_t* list, int n) {
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += NT) list[i] = ~0ull;
-    __syncthreads();
+// The thinking warp's functions are called, not inlined, and their loops not
+// unrolled: a row passes through all of this code once, so its length is what
+// the instruction cache has to bring in for every row.
+
+// One warp sorts the first c <= kList entries of the list.
+__device__ __noinline__ void sort_list(SampleShared& s, int c) {
+    const int lane = threadIdx.x & 31;
+    int size = 32;
+    while (size < c) size *= 2;
+    for (int i = c + lane; i < size; i += 32) s.list[i] = ~0ull;
+    __syncwarp();
+#pragma unroll 1
     for (int k = 2; k <= size; k *= 2)
+#pragma unroll 1
         for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = threadIdx.x; t < size / 2; t += NT) {
+#pragma unroll 1
+            for (int t = lane; t < size / 2; t += 32) {
                 const int i = 2 * t - (t & (j - 1));
-                const uint64_t a = list[i], b = list[i + j];
+                const uint64_t a = s.list[i], b = s.list[i + j];
                 if ((a > b) == ((i & k) == 0)) {
-                    list[i] = b;
-                    list[i + j] = a;
+                    s.list[i] = b;
+                    s.list[i + j] = a;
                 }
             }
-            // strides up to 32 stay within a warp's 64 entries
-            if (j > 32 || j == 1) __syncthreads(); else __syncwarp();
+            __syncwarp();
         }
 }
+// Prefixes before each lane's 16 buckets.
+__device__ __noinline__ void lane_prefixes(SampleShared& s, int level) {
+    const int lane = threadIdx.x & 31;
+    uint64_t w = 0;
+    uint32_t k = 0;
+    const ulonglong2* ms = reinterpret_cast<const ulonglong2*>(&s.mass[level][lane * kPerLane]);
+    const uint4* ts = reinterpret_cast<const uint4*>(&s.tokens[level][lane * kPerLane]);
+#pragma unroll
+    for (int i = 0; i < kPerLane / 2; ++i) w += ms[i].x + ms[i].y;
+#pragma unroll
+    for (int i = 0; i < kPerLane / 4; ++i) k += ts[i].x + ts[i].y + ts[i].z + ts[i].w;
+    const uint64_t ws = warp_scan(w);
+    const uint32_t ks = uint32_t(warp_scan(k));
+    s.lane_mass[level][lane] = ws - w;
+    s.lane_tokens[level][lane] = ks - k;
+    if (lane == 31) {
+        s.lane_mass[level][32] = ws;
+        s.lane_tokens[level][32] = ks;
+    }
+    __syncwarp();
+}
+struct Bucket {
+    int at;
+    uint64_t mass;  // before it
+    uint32_t count;
+};
+// The bucket in which the prefix exceeds `want` (which lies in one).
+__device__ __noinline__ Bucket find_bucket(const SampleShared& s, int level, bool counted, uint64_t want) {
+    const int lane = threadIdx.x & 31;
+    const bool here = counted ? s.lane_tokens[level][lane] <= want && want < s.lane_tokens[level][lane + 1]
+                              : s.lane_mass[level][lane] <= want && want < s.lane_mass[level][lane + 1];
+    const int src = (__ffs(__ballot_sync(0xffffffffu, here)) - 1) & 31;
+    const int b = src * kPerLane + (lane & (kPerLane - 1));
+    const uint64_t w = lane < kPerLane ? s.mass[level][b] : 0;
+    const uint32_t k = lane < kPerLane ? s.tokens[level][b] : 0;
+    const uint64_t we = s.lane_mass[level][src] + warp_scan(w);
+    const uint32_t ke = s.lane_tokens[level][src] + uint32_t(warp_scan(k));
+    const int at = (__ffs(__ballot_sync(0xffffffffu, lane < kPerLane && want < (counted ? uint64_t(ke) : we))) - 1) & 31;
+    return {src * kPerLane + at, __shfl_sync(0xffffffffu, we - w, at), __shfl_sync(0xffffffffu, ke - k, at)};
+}
+struct Found {
+    uint64_t entry, prefix;  // the prefix mass with the entry
+};
+// Where the prefix of the sorted list's entries [from, to) exceeds `want`, given
+// the mass and the count before them.
+__device__ __noinline__ Found find_in_list(const SampleShared& s, int from, int to, uint64_t w0, uint64_t k0, bool counted,
+                                           uint64_t want) {
+    const int lane = threadIdx.x & 31;
+    uint64_t e = 0, prefix = 0;
+    unsigned hit = 0;
+#pragma unroll 1
+    for (int j0 = from; j0 < to && !hit; j0 += 32) {
+        const int j = j0 + lane;
+        e = j < to ? s.list[j] : 0;
+        const uint32_t w = j < to ? mass_of_key(uint32_t(e >> 32)) : 0u;
+        prefix = w0 + warp_scan(w);
+        hit = __ballot_sync(0xffffffffu, j < to && (counted ? k0 + (j - from) == want : want < prefix && want >= prefix - w));
+        w0 = __shfl_sync(0xffffffffu, prefix, 31);
+    }
+    const int src = (__ffs(hit) - 1) & 31;
+    return {__shfl_sync(0xffffffffu, e, src), __shfl_sync(0xffffffffu, prefix, src)};
+}
+// The first entry of the sorted list with a key >= `key`.
+__device__ __forceinline__ int list_from(const SampleShared& s, int c, uint32_t key) {
+    int at = 0;
+#pragma unroll 1
+    for (int j0 = 0; j0 < c; j0 += 32) {
+        const int j = j0 + (threadIdx.x & 31);
+        at += __popc(__ballot_sync(0xffffffffu, j < c && uint32_t(s.list[j] >> 32) < key));
+    }
+    return at;
+}
 
-// One block per row, or a cluster of them with a slice each; the slice is held in
-// shared memory as y.  The first CTA decides, the others follow its commands.
-// Every pass over a slice costs less than its load did; what a row takes beside
-// them is the latency of the block's (and the cluster's) barriers, so few rows to
-// an SM overlap.
+// One block per row, or a cluster of them with a slice each, held in shared memory.
+// The first warp of the first CTA thinks, all others make the passes that it asks
+// for: a histogram, the collection of a bucket's tokens, rarely the nth of equal
+// tokens.  Most tokens lie far below the largest (beyond y = 8): the first pass
+// gives them no buckets, only their sum.
 template <class T, int NT>
-__global__ void __launch_bounds__(NT)
-sample_kernel(const SampleArgs a, int slices, int held)
+__global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8)
+sample_kernel(const SampleArgs a, int slices, int log_slices)
 {
     HX_PDL_PROLOGUE();
     extern __shared__ __align__(16) uint8_t smem[];
     SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
-    float* y = reinterpret_cast<float*>(smem + ((sizeof(SampleShared) + 15) & ~size_t(15)));  // [held]
+    uint4* held = reinterpret_cast<uint4*>(smem + ((sizeof(SampleShared) + 15) & ~size_t(15)));
     constexpr int EPV = Chunk<T>::EPV;
     const int tid = threadIdx.x, lane = tid & 31, V = int(a.vocab);
     const int rank = int(blockIdx.x) & (slices - 1);
-    const size_t row = blockIdx.x / unsigned(slices);
+    const size_t row = blockIdx.x >> log_slices;
     const T* l = static_cast<const T*>(a.logits) + row * a.stride;
-    const bool many = slices > 1;
+    const bool many = slices > 1, thinker = rank == 0 && tid < 32;
     auto sync = [&] {
         if (many) tc::cluster_sync(); else __syncthreads();
     };
-    // this CTA's chunks; y[p] is element p + base
     const int lead = int((reinterpret_cast<uintptr_t>(l) & 15) / sizeof(T));
-    const int chunks = (V + lead + EPV - 1) / EPV, each = (chunks + slices - 1) / slices;
-    const int first = min(chunks, rank * each), last = min(chunks, first + each);
-    const int base = first * EPV - lead, n = (last - first) * EPV;
+    const int chunks = (V + lead + EPV - 1) / EPV, each = (chunks + slices - 1) >> log_slices;
+    const int first = min(chunks, rank * each), n = min(chunks, first + each) - first;  // this CTA's chunks
+    const int base = first * EPV - lead;                                                // element 0 of chunk 0
 
-    // ---- the slice, its maximum ----
-    if (tid == 0) s.nan = 0;
+    // ---- the slice and its maximum ----
     float m = -INFINITY;
-    bool nan = false;
-    for (int c0 = first + tid; c0 < last; c0 += 4 * NT) {
+    auto keep = [&](int c, const uint4& raw) {
+        held[c] = raw;
+        m = max_or_nan(m, chunk_max(raw, T()));
+    };
+    const float uniform = thinker ? a.uniform[row] : 0.f;
+    const int whole0 = lead > 0 && first == 0 ? 1 : 0, whole1 = max(whole0, min(n, (V + lead) / EPV - first));
+    const uint4* from = reinterpret_cast<const uint4*>(l - lead) + first;
+    for (int c0 = whole0 + tid; c0 < whole1; c0 += 4 * NT) {
         uint4 raw[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int i = (c0 + q * NT) * EPV - lead;
-            if (c0 + q * NT < last && i >= 0 && i + EPV <= V) raw[q] = *reinterpret_cast<const uint4*>(l + i);
-        }
+        for (int q = 0; q < 4; ++q)
+            if (c0 + q * NT < whole1) raw[q] = from[c0 + q * NT];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int c = c0 + q * NT, i = c * EPV - lead;
-            if (c >= last) break;
+        for (int q = 0; q < 4; ++q)
+            if (c0 + q * NT < whole1) keep(c0 + q * NT, raw[q]);
+    }
+    // the chunks that begin before the row or end after it
+    if (tid < 2) {
+        const int c = tid == 0 ? 0 : n - 1;
+        if (n > 0 && (tid == 0 ? whole0 == 1 : whole1 < n && (c > 0 || whole0 == 0))) {
             float x[EPV];
-            if (i >= 0 && i + EPV <= V) {
-                Chunk<T>::unpack(raw[q], x);
-            } else {
-#pragma unroll
-                for (int r = 0; r < EPV; ++r) x[r] = i + r >= 0 && i + r < V ? to_float(l[i + r]) : -INFINITY;
-            }
 #pragma unroll
             for (int r = 0; r < EPV; ++r) {
-                nan |= x[r] != x[r];
-                m = fmaxf(m, x[r]);
+                const int i = base + c * EPV + r;
+                x[r] = i >= 0 && i < V ? to_float(l[i]) : -INFINITY;
             }
-            float4* to = reinterpret_cast<float4*>(y + (c - first) * EPV);
-#pragma unroll
-            for (int r = 0; r < EPV; r += 4) to[r / 4] = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
+            keep(c, Chunk<T>::pack(x));
         }
     }
-    float* scratch = reinterpret_cast<float*>(s.scan);
-    m = block_reduce<NT>(m, scratch, MaxOp());
-    nan = __syncthreads_or(nan || m == INFINITY) != 0;
+    bool nan = __syncthreads_or(!(m < INFINITY)) != 0;
+    m = block_reduce<NT>(m, reinterpret_cast<float*>(s.scan), MaxOp());
     if (many) {
         tc::cluster_sync();  // every CTA has started
-        // a NaN marks the whole row: no maximum is above it
-        if (tid < slices) {
-            const uint32_t to = tc::cluster_addr(&s.maxima[rank], tid);
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(nan ? INFINITY : m) : "memory");
-        }
+        // a NaN marks the whole row: no maximum is above +inf
+        if (tid < slices)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(tc::cluster_addr(&s.maxima[rank], tid)),
+                         "f"(nan ? INFINITY : m) : "memory");
         tc::cluster_sync();
         for (int r = 0; r < slices; ++r) m = fmaxf(m, s.maxima[r]);
         nan = m == INFINITY;
@@ -230,99 +328,326 @@ sample_kernel(const SampleArgs a, int slices, int held)
     }
 
     const float temp = a.temperature ? a.temperature[row] : 1.f;
-    float inv_t = __fdiv_rn(1.f, temp);
-    const bool greedy = !(temp > 0.f) || temp == INFINITY || inv_t == INFINITY;
-    if (greedy) inv_t = 1.f;
-    int top_k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
-    if (top_k <= 0 || top_k >= V) top_k = 0;
-    const float p = a.top_p && !greedy ? a.top_p[row] : 1.f, mp = a.min_p && !greedy ? a.min_p[row] : 0.f;
-    const float limit = mp > 0.f ? fmaxf(-logf(mp), 0.f) : INFINITY;
-
-    for (int i = tid * 4; i < n; i += NT * 4) {
-        float4 x = *reinterpret_cast<float4*>(y + i);
-        x.x = __fmul_rn(__fsub_rn(m, x.x), inv_t);
-        x.y = __fmul_rn(__fsub_rn(m, x.y), inv_t);
-        x.z = __fmul_rn(__fsub_rn(m, x.z), inv_t);
-        x.w = __fmul_rn(__fsub_rn(m, x.w), inv_t);
-        *reinterpret_cast<float4*>(y + i) = x;
+    const float inv_t = __fdiv_rn(1.f, temp);
+    if (!(temp > 0.f) || temp == INFINITY || inv_t == INFINITY) {  // the first largest logit
+        int at = 0x7fffffff;
+        for (int c = tid; c < n; c += NT) {
+            float x[EPV];
+            Chunk<T>::unpack(held[c], x);
+#pragma unroll
+            for (int r = 0; r < EPV; ++r)
+                if (x[r] == m) at = min(at, base + c * EPV + r);
+        }
+        at = -block_reduce<NT>(-at, reinterpret_cast<int*>(s.scan), MaxOp());
+        if (many) {
+            if (tid == 0)
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.nth_counts[rank], 0)), "r"(at)
+                             : "memory");
+            tc::cluster_sync();
+            if (rank == 0)
+                for (int r = 0; r < slices; ++r) at = min(at, int(s.nth_counts[r]));
+        }
+        if (tid == 0 && rank == 0) {
+            a.tokens[row] = at;
+            if (a.log_probs) a.log_probs[row] = 0.f;
+        }
+        return;  // the whole cluster
     }
+    const int top_k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f;
+    const float limit = mp > 0.f ? fmaxf(-logf(mp), 0.f) : INFINITY;
+    const bool whole = top_k <= 0 || (mp > 0.f && limit > 8.f);
 
-    // ---- the commands ----
-    // bucket of a key under (lo, shift): the first takes all below its range
-    const uint32_t first_lo = kTopKey - (uint32_t(kBuckets) << kFirstShift);
-    auto bucket_of = [](uint32_t key, uint32_t lo, int shift) { return key < lo ? 0u : (key - lo) >> shift; };
-    auto histogram = [&](const SampleCommand& c, bool with_limit) {
-        for (int b = tid; b < kBuckets; b += NT) s.low[b] = s.high[b] = s.count[b] = 0u;
-        __syncthreads();
-        uint64_t below = 0;
-        const uint32_t from = with_limit ? first_lo : c.lo;
-        for (int i = tid; i < n; i += NT) {
-            const float v = y[i];
-            const uint32_t key = __float_as_uint(v);
-            if (key >= c.hi || (!with_limit && key < c.lo)) continue;
-            const uint32_t w = mass_of(v);
-            if (w == 0) continue;
-            const uint32_t b = bucket_of(key, from, c.shift);
-            atomicAdd(&s.low[b], w & 0xffffu);
-            atomicAdd(&s.high[b], w >> 16);
-            atomicAdd(&s.count[b], 1u);
-            if (v <= limit) below += w;
+    // Goes on until a pass over the row is needed.
+    auto think = [&](bool begin) {
+        Thought t;
+        if (begin) {
+            t = Thought{};
+            t.pending = -1;
+            t.least = ~0ull;
+        } else {
+            t = s.thought;
         }
-        if (with_limit && mp > 0.f) {
-            below = block_reduce<NT>(below, s.scan, SumOp());
-            if (tid == 0) {
-                if (many) remote_store(tc::cluster_addr(&s.min_mass[rank], 0), below); else s.min_mass[0] = below;
+        auto ask = [&](int step, uint32_t lo, uint32_t hi, uint32_t lo2, uint32_t hi2, int shift, uint32_t nth, int sums) {
+            t.pending = sums ? -2 : step;
+            __syncwarp();
+            if (lane == 0) {
+                s.command = {step, lo, hi, lo2, hi2, shift, nth, sums ? 0 : 1, sums};
+                s.listed = 0;
+                s.thought = t;
             }
-        }
-        sync();
-        // the buckets of all slices, each CTA a share of them, to the first CTA
-        const int level = with_limit ? 0 : 1, share = kBuckets / slices;
-        for (int b = rank * share + tid; b < (rank + 1) * share; b += NT) {
-            uint64_t w = 0;
-            uint32_t k = 0;
-            for (int r = 0; r < slices; ++r) {
-                if (many) {
-                    w += (uint64_t(remote_u32(tc::cluster_addr(&s.high[b], r))) << 16) +
-                         remote_u32(tc::cluster_addr(&s.low[b], r));
-                    k += remote_u32(tc::cluster_addr(&s.count[b], r));
-                } else {
-                    w += (uint64_t(s.high[b]) << 16) + s.low[b];
-                    k += s.count[b];
+        };
+        auto collect = [&](uint32_t lo, uint32_t hi, uint32_t lo2, uint32_t hi2) { ask(kCollect, lo, hi, lo2, hi2, 0, 0, 0); };
+        auto finer = [&] {
+            t.refine_shift = 0;
+            while (((t.hi - 1 - t.lo) >> t.refine_shift) >= uint32_t(kBuckets)) ++t.refine_shift;
+            ask(kHistogram, t.lo, t.hi, t.lo, 0, t.refine_shift, 0, 0);
+        };
+        auto bucket_lo = [](int b) { return b == 0 ? 0u : kFirstKey + (uint32_t(b) << kFirstShift); };
+        auto bucket_hi = [](int b) { return kFirstKey + (uint32_t(b + 1) << kFirstShift); };
+        const uint64_t u = min(fraction32(uniform), uint64_t(0xffffffffu)), p32 = fraction32(p);
+        Found found{};
+        bool have = false;  // `found` answers the goal
+        if (begin) lane_prefixes(s, 0);
+        const uint64_t head_mass = s.lane_mass[0][32];
+        const uint32_t head_tokens = s.lane_tokens[0][32];
+        if (t.pending < 0) {
+            if (begin && !whole && uint32_t(top_k) > head_tokens) {  // the first k reach beyond the first histogram
+                ask(kHistogram, 0, kHeadKey, kFirstKey, 0, kFirstShift, 0, 1);
+                return;
+            }
+            t.total = head_mass;
+            t.tokens = head_tokens;
+            if (whole || t.pending == -2)
+                for (int r = 0; r < slices; ++r) {
+                    t.total += s.rest_mass[r];
+                    t.tokens += s.rest_tokens[r];
+                }
+            if (mp > 0.f) {
+                t.least = 0;
+                for (int r = 0; r < slices; ++r) t.least += s.min_mass[r];
+            }
+            t.W = t.total;
+            const bool counted = top_k > 0 && uint32_t(top_k) <= t.tokens;
+            t.goal = counted ? kTopK : p < 1.f ? kTopP : kToken;
+            // all that will be asked lies below this: where few tokens do, they
+            // are collected once
+            const uint64_t most = counted ? uint64_t(top_k) - 1
+                                  : p < 1.f ? scaled_mass(t.total, p32) : scaled_mass(min(t.least, t.total), u);
+            if (counted ? most < head_tokens : most < head_mass) {
+                const Bucket b = find_bucket(s, 0, counted, most);
+                if (b.count + s.tokens[0][b.at] <= uint32_t(kList)) {
+                    t.head = true;
+                    collect(0, bucket_hi(b.at), 0, 0);
+                    return;
                 }
             }
-            if (many) {
-                remote_store(tc::cluster_addr(&s.mass[level][b], 0), w);
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.tokens[level][b], 0)), "r"(k)
-                             : "memory");
-            } else {
-                s.mass[level][b] = w;
-                s.tokens[level][b] = k;
+        } else if (t.head && t.head_count == 0) {
+            t.head_count = int(s.listed);
+            sort_list(s, t.head_count);
+        } else if (t.pending == kCollect) {
+            const int c = int(s.listed);
+            if (c > kList) {
+                if (t.planned) {  // together too many: one after the other
+                    t.planned = false;
+                    collect(t.lo, t.hi, 0, 0);
+                } else {
+                    finer();
+                }
+                return;
+            }
+            sort_list(s, c);
+            const bool apart = t.planned && t.plan_hi <= t.lo;
+            const int from = apart ? list_from(s, c, t.lo) : 0;
+            found = find_in_list(s, from, c, t.mass, t.count, t.by_count, t.amount);
+            have = true;
+            if (t.planned) {  // the token that follows lies in the list too
+                t.W = min(found.prefix, t.least);
+                t.goal = kToken;
+                found = find_in_list(s, 0, apart ? from : c, t.plan_mass, 0, false, scaled_mass(t.W, u));
             }
         }
-        sync();
-    };
-    auto collect = [&](const SampleCommand& c) {
-        const uint32_t counter = many ? tc::cluster_addr(&s.listed, 0) : 0, list = many ? tc::cluster_addr(s.list, 0) : 0;
-        for (int i = tid; i < n; i += NT) {
-            const uint32_t key = __float_as_uint(y[i]);
-            if (key < c.lo || key >= c.hi) continue;
-            const uint64_t entry = (uint64_t(key) << 32) | uint32_t(i + base);
-            if (many) {
-                const uint32_t at = remote_add(counter, 1u);
-                if (at < kList) remote_store(list + at * 8, entry);
-            } else {
-                const uint32_t at = atomicAdd(&s.listed, 1u);
-                if (at < kList) s.list[at] = entry;
+#pragma unroll 1
+        for (;;) {
+            if (!have) {
+                if (t.pending == kHistogram) {  // continue within [lo, hi)
+                    lane_prefixes(s, 1);
+                    const Bucket b = find_bucket(s, 1, t.by_count, t.by_count ? t.amount - t.count : t.amount - t.mass);
+                    t.mass += b.mass;
+                    t.count += b.count;
+                    t.hi = min(t.hi, t.lo + (uint32_t(b.at + 1) << t.refine_shift));
+                    t.lo += uint32_t(b.at) << t.refine_shift;
+                } else {  // a new goal
+                    t.by_count = t.goal == kTopK;
+                    if (t.goal == kTopK) {
+                        t.amount = uint64_t(top_k) - 1;
+                    } else if (t.goal == kTopP) {
+                        const uint64_t need = scaled_mass(t.W, p32);
+                        t.amount = need < 1 ? 0 : need - 1;
+                    } else {
+                        t.W = min(t.W, t.least);
+                        t.amount = scaled_mass(t.W, u);
+                    }
+                    if (t.head) {
+                        found = find_in_list(s, 0, t.head_count, 0, 0, t.by_count, t.amount);
+                        have = true;
+                    } else if (t.by_count ? t.amount < head_tokens : t.amount < head_mass) {
+                        const Bucket b = find_bucket(s, 0, t.by_count, t.amount);
+                        t.lo = bucket_lo(b.at);
+                        t.hi = bucket_hi(b.at);
+                        t.mass = b.mass;
+                        t.count = b.count;
+                        t.planned = false;
+                        if (t.goal == kTopP || (t.goal == kTopK && !(p < 1.f))) {
+                            // W will lie in this bucket: but for that the token's bucket is
+                            // known, and its tokens are collected in the same pass
+                            const Bucket b1 = find_bucket(s, 0, false, scaled_mass(min(b.mass, t.least), u));
+                            const Bucket b2 = find_bucket(s, 0, false, scaled_mass(min(b.mass + s.mass[0][b.at], t.least), u));
+                            if (b2.count + s.tokens[0][b2.at] - b1.count + s.tokens[0][b.at] <= uint32_t(kList)) {
+                                t.planned = true;
+                                t.plan_mass = b1.mass;
+                                t.plan_hi = bucket_hi(b2.at);
+                                if (b2.at < b.at) {
+                                    collect(t.lo, t.hi, bucket_lo(b1.at), t.plan_hi);
+                                    return;
+                                }
+                                // one interval: the list begins at the token's first bucket
+                                t.lo = bucket_lo(b1.at);
+                                t.mass = b1.mass;
+                                t.count = b1.count;
+                            }
+                        }
+                    } else {  // beyond the first histogram
+                        t.mass = head_mass;
+                        t.count = head_tokens;
+                        t.lo = kHeadKey;
+                        t.hi = kTopKey;
+                        finer();
+                        return;
+                    }
+                }
+                if (!have) {
+                    if (t.hi - t.lo > 1) {
+                        collect(t.lo, t.hi, 0, 0);
+                        return;
+                    }
+                    // one key: its tokens have one mass
+                    const uint64_t w = mass_of_key(t.lo);
+                    const uint64_t nth = t.by_count ? t.amount - t.count : (t.amount - t.mass) / w;
+                    found.prefix = t.mass + (nth + 1) * w;
+                    if (t.goal == kToken) {
+                        found.entry = uint64_t(t.lo) << 32;
+                        t.amount = nth;
+                    }
+                }
             }
+            if (t.goal == kToken) {
+                if (lane == 0) {
+                    if (have) a.tokens[row] = int32_t(uint32_t(found.entry));
+                    if (a.log_probs)
+                        a.log_probs[row] = -__uint_as_float(uint32_t(found.entry >> 32)) -
+                                           logf(float(t.W) * (1.f / 2147483648.f));
+                }
+                ask(have ? kDone : kNth, t.lo, t.lo + 1, 0, 0, 0, uint32_t(t.amount), 0);
+                return;
+            }
+            have = false;
+            t.pending = kDone;
+            t.W = found.prefix;
+            t.goal = t.goal == kTopK && p < 1.f ? kTopP : kToken;
+        }
+    };
+
+    // ---- passes, the first a histogram up to y = 8 with, where the filters need
+    // it, the sum of the rest ----
+    SampleCommand cmd{kHistogram, 0, kHeadKey, kFirstKey, 0, kFirstShift, 0, 0, whole};
+    const T* element = reinterpret_cast<const T*>(held);
+    auto y_of = [&](int i) { return __fmul_rn(__fsub_rn(m, to_float(element[i])), inv_t); };
+#pragma unroll 1
+    for (bool begin = true;; begin = false) {
+        // a logit below which no key is below hi: y >= hi once (m - l)/T is above it
+        // by more than the roundings
+        const float least = m - __uint_as_float(cmd.hi) * temp * 1.00001f - fabsf(m) * 1e-5f;
+        if (cmd.step == kHistogram) {
+            for (int b = tid; b < kBuckets; b += NT) s.low[b] = s.high[b] = s.count[b] = 0u;
+            __syncthreads();
+            uint64_t rest = 0, below = 0;
+            uint32_t tokens = 0;
+#pragma unroll 1
+            for (int c = tid; c < n; c += NT) {
+                const uint4 raw = held[c];
+                if (!cmd.sums && !(chunk_max(raw, T()) >= least)) continue;
+                float x[EPV];
+                Chunk<T>::unpack(raw, x);
+#pragma unroll
+                for (int r = 0; r < EPV; ++r) {
+                    const float y = __fmul_rn(__fsub_rn(m, x[r]), inv_t);
+                    const uint32_t key = __float_as_uint(y), w = mass_of(y);
+                    if (key - cmd.lo < cmd.hi - cmd.lo) {
+                        if (w) {
+                            const uint32_t b = key < cmd.lo2 ? 0u : (key - cmd.lo2) >> cmd.shift;
+                            atomicAdd(&s.low[b], w & 0xffffu);
+                            atomicAdd(&s.high[b], w >> 16);
+                            atomicAdd(&s.count[b], 1u);
+                        }
+                    } else if (key >= kHeadKey) {
+                        rest += w;
+                        tokens += w != 0;
+                    }
+                    if (y <= limit) below += w;
+                }
+            }
+            if (cmd.level == 0) {  // the slice's sums to the first CTA
+                rest = block_reduce<NT>(rest, s.scan, SumOp());
+                below = block_reduce<NT>(below, s.scan, SumOp());
+                tokens = block_reduce<NT>(tokens, reinterpret_cast<uint32_t*>(s.scan), SumOp());
+                if (tid == 0) {
+                    if (many) {
+                        remote_store(tc::cluster_addr(&s.rest_mass[rank], 0), rest);
+                        remote_store(tc::cluster_addr(&s.min_mass[rank], 0), below);
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.rest_tokens[rank], 0)),
+                                     "r"(tokens) : "memory");
+                    } else {
+                        s.rest_mass[0] = rest;
+                        s.min_mass[0] = below;
+                        s.rest_tokens[0] = tokens;
+                    }
+                }
+            }
+            sync();
+            // the buckets of all slices, each CTA a share of them, to the first CTA
+            const int share = kBuckets >> log_slices;
+#pragma unroll 1
+            for (int b = rank * share + tid; b < (rank + 1) * share; b += NT) {
+                if (many) {
+                    uint64_t w = 0;
+                    uint32_t k = 0;
+                    for (int r = 0; r < slices; ++r) {
+                        w += (uint64_t(remote_u32(tc::cluster_addr(&s.high[b], r))) << 16) +
+                             remote_u32(tc::cluster_addr(&s.low[b], r));
+                        k += remote_u32(tc::cluster_addr(&s.count[b], r));
+                    }
+                    remote_store(tc::cluster_addr(&s.mass[cmd.level][b], 0), w);
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.tokens[cmd.level][b], 0)),
+                                 "r"(k) : "memory");
+                } else {
+                    s.mass[cmd.level][b] = (uint64_t(s.high[b]) << 16) + s.low[b];
+                    s.tokens[cmd.level][b] = s.count[b];
+                }
+            }
+        } else if (cmd.step == kCollect) {
+            const uint32_t counter = many ? tc::cluster_addr(&s.listed, 0) : 0, list = many ? tc::cluster_addr(s.list, 0) : 0;
+#pragma unroll 1
+            for (int c = tid; c < n; c += NT) {
+                if (!(chunk_max(held[c], T()) >= least)) continue;
+#pragma unroll 1
+                for (int i = c * EPV; i < (c + 1) * EPV; ++i) {
+                    const uint32_t key = __float_as_uint(y_of(i));
+                    if (key - cmd.lo >= cmd.hi - cmd.lo && key - cmd.lo2 >= cmd.hi2 - cmd.lo2) continue;
+                    const uint64_t entry = (uint64_t(key) << 32) | uint32_t(base + i);
+                    const uint32_t at = many ? remote_add(counter, 1u) : atomicAdd(&s.listed, 1u);
+                    if (at >= kList) continue;
+                    if (many) remote_store(list + at * 8, entry); else s.list[at] = entry;
+                }
+            }
+        } else {
+            break;
         }
         sync();
-    };
-    // the token that is the nth with key lo, in index order
-    auto nth_token = [&](const SampleCommand& c) {
-        uint32_t mine = 0;
-        for (int i = tid; i < n; i += NT) mine += __float_as_uint(y[i]) == c.lo;
+        if (thinker) think(begin);
+        sync();
+        if (rank == 0) {
+            cmd = s.command;
+        } else {
+            const uint32_t at = tc::cluster_addr(&s.command, 0);
+            cmd = {int(remote_u32(at)), remote_u32(at + 4), remote_u32(at + 8), remote_u32(at + 12), remote_u32(at + 16),
+                   int(remote_u32(at + 20)), remote_u32(at + 24), int(remote_u32(at + 28)), int(remote_u32(at + 32))};
+        }
+    }
+    if (cmd.step == kNth) {  // the nth token with key lo, in index order
+        uint32_t mine = 0, before = 0;
+        for (int i = tid; i < n * EPV; i += NT) mine += __float_as_uint(y_of(i)) == cmd.lo;
         mine = block_reduce<NT>(mine, reinterpret_cast<uint32_t*>(s.scan), SumOp());
-        uint32_t before = 0;
         if (many) {
             if (tid < slices)
                 asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.nth_counts[rank], tid)), "r"(mine)
@@ -330,231 +655,34 @@ sample_kernel(const SampleArgs a, int slices, int held)
             tc::cluster_sync();
             for (int r = 0; r < rank; ++r) before += s.nth_counts[r];
         }
-        if (c.nth < before || c.nth >= before + mine) return;
-        uint32_t have = before;
-        uint32_t* votes_of = reinterpret_cast<uint32_t*>(s.scan);
-        for (int i0 = 0; i0 < n && have <= c.nth; i0 += NT) {
-            const int i = i0 + tid;
-            const bool eq = i < n && __float_as_uint(y[i]) == c.lo;
-            const unsigned votes = __ballot_sync(0xffffffffu, eq);
-            if (lane == 0) votes_of[tid >> 5] = __popc(votes);
-            __syncthreads();
-            uint32_t at = have;
-            for (int w = 0; w < NT / 32; ++w) {
-                if (w < (tid >> 5)) at += votes_of[w];
-                have += votes_of[w];
+        if (cmd.nth >= before && cmd.nth < before + mine) {
+            uint32_t have = before;
+            uint32_t* votes_of = reinterpret_cast<uint32_t*>(s.scan);
+#pragma unroll 1
+            for (int i0 = 0; i0 < n * EPV && have <= cmd.nth; i0 += NT) {
+                const int i = i0 + tid;
+                const bool eq = i < n * EPV && __float_as_uint(y_of(i)) == cmd.lo;
+                const unsigned votes = __ballot_sync(0xffffffffu, eq);
+                if (lane == 0) votes_of[tid >> 5] = __popc(votes);
+                __syncthreads();
+                uint32_t at = have;
+                for (int w = 0; w < NT / 32; ++w) {
+                    if (w < (tid >> 5)) at += votes_of[w];
+                    have += votes_of[w];
+                }
+                at += __popc(votes & ((1u << lane) - 1));
+                if (eq && at == cmd.nth) a.tokens[row] = base + i;
+                __syncthreads();
             }
-            at += __popc(votes & ((1u << lane) - 1));
-            if (eq && at == c.nth) a.tokens[row] = i + base;
-            __syncthreads();
-        }
-    };
-
-    // The first histogram needs no command.
-    SampleCommand cmd{kHistogram, first_lo, kTopKey, kFirstShift, 0};
-    histogram(cmd, true);
-    if (rank != 0) {
-        for (;;) {
-            tc::cluster_sync();
-            const uint32_t at = tc::cluster_addr(&s.command, 0);
-            cmd.step = int(remote_u32(at));
-            cmd.lo = remote_u32(at + 4);
-            cmd.hi = remote_u32(at + 8);
-            cmd.shift = int(remote_u32(at + 12));
-            cmd.nth = remote_u32(at + 16);
-            if (cmd.step == kHistogram) histogram(cmd, false);
-            else if (cmd.step == kCollect) collect(cmd);
-            else {
-                if (cmd.step == kNth) nth_token(cmd);
-                break;
-            }
-        }
-        tc::cluster_sync();
-        return;
-    }
-
-    // ---- the first CTA ----
-    auto issue = [&](const SampleCommand& c) {
-        if (tid == 0) {
-            s.command = c;
-            s.listed = 0;
-        }
-        sync();
-    };
-    // turns bucket masses and counts into prefixes before each bucket
-    auto prefixes = [&](int level) {
-        constexpr int per = kBuckets / NT;
-        uint64_t w[per], sum = 0;
-        uint32_t k[per], count = 0;
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-            w[i] = s.mass[level][tid * per + i];
-            k[i] = s.tokens[level][tid * per + i];
-            sum += w[i];
-            count += k[i];
-        }
-        uint64_t total, all;
-        uint64_t at = block_scan<NT>(sum, s.scan, total) - sum;
-        uint32_t c = uint32_t(block_scan<NT>(count, s.scan, all)) - count;
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-            s.mass[level][tid * per + i] = at;
-            s.tokens[level][tid * per + i] = c;
-            at += w[i];
-            c += k[i];
-        }
-        if (tid == 0) s.total[level] = total;
-        __syncthreads();
-        return uint32_t(all);
-    };
-    const uint32_t positive = prefixes(0);  // tokens with mass
-    const uint64_t total = s.total[0];
-    auto mass_after = [&](int level, int b) { return b + 1 < kBuckets ? s.mass[level][b + 1] : s.total[level]; };
-
-    struct Place {       // where a prefix crosses an amount
-        uint32_t key;    // of the token
-        int index;       // of the token; -1 when only its number among its equals is known
-        uint32_t nth;
-        uint64_t prefix; // mass up to and with the token
-    };
-    // the bucket that holds the token: by mass, or by number of tokens
-    auto find_bucket = [&](int level, bool by_count, uint64_t amount) {
-        for (int b = tid; b < kBuckets; b += NT) {
-            const uint64_t at = by_count ? s.tokens[level][b] : s.mass[level][b];
-            const uint64_t to = b + 1 < kBuckets ? (by_count ? s.tokens[level][b + 1] : s.mass[level][b + 1])
-                                                 : (by_count ? ~0ull : s.total[level]);
-            if (at <= amount && amount < to && (!by_count || b + 1 < kBuckets || s.mass[level][b] < s.total[level])) {
-                s.found_bucket = b;
-                s.found_mass = s.mass[level][b];
-                s.found_count = s.tokens[level][b];
-            }
-        }
-        __syncthreads();
-        const int b = int(s.found_bucket);
-        return b;
-    };
-    // within the sorted list of c tokens, mass and count before it given
-    auto find_in_list = [&](int c, uint64_t mass, uint64_t count, bool by_count, uint64_t amount) {
-        constexpr int per = kList / NT;
-        uint64_t e[per], w[per], sum = 0;
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-            const int at = tid * per + i;
-            e[i] = at < c ? s.list[at] : 0ull;
-            w[i] = at < c ? mass_of_key(uint32_t(e[i] >> 32)) : 0u;
-            sum += w[i];
-        }
-        uint64_t all;
-        uint64_t at = mass + block_scan<NT>(sum, s.scan, all) - sum;
-#pragma unroll
-        for (int i = 0; i < per; ++i) {
-            const int j = tid * per + i;
-            const bool here = by_count ? count + j == amount : at <= amount && amount < at + w[i];
-            if (j < c && here) {
-                s.found_mass = at + w[i];
-                s.found_bucket = uint32_t(e[i] >> 32);
-                s.found_count = uint32_t(e[i]);
-            }
-            at += w[i];
-        }
-        __syncthreads();
-        Place r{s.found_bucket, int(s.found_count), 0, s.found_mass};
-        __syncthreads();
-        return r;
-    };
-    bool head = false;  // the list holds the head of the order, sorted
-    int head_count = 0;
-    auto cross = [&](bool by_count, uint64_t amount) {
-        if (head) return find_in_list(head_count, 0, 0, by_count, amount);
-        int level = 0, b = find_bucket(0, by_count, amount), shift = kFirstShift;
-        uint64_t mass = s.found_mass;
-        uint64_t count = s.found_count;
-        uint32_t lo = b == 0 ? 0u : first_lo + (uint32_t(b) << shift), hi = first_lo + (uint32_t(b + 1) << shift);
-        __syncthreads();
-        for (;;) {
-            if (hi - lo == 1) {  // one key: its tokens have one mass
-                const uint64_t w = mass_of_key(lo);
-                const uint64_t nth = by_count ? amount - count : (amount - mass) / w;
-                return Place{lo, -1, uint32_t(nth), mass + (nth + 1) * w};
-            }
-            issue({kCollect, lo, hi, 0, 0});
-            collect({kCollect, lo, hi, 0, 0});
-            const int c = int(s.listed);
-            if (c <= kList) {
-                block_sort<NT>(s.list, c);
-                return find_in_list(c, mass, count, by_count, amount);
-            }
-            // too many: a finer histogram of this bucket
-            shift = 0;
-            while (((hi - 1 - lo) >> shift) >= uint32_t(kBuckets)) ++shift;
-            const SampleCommand finer{kHistogram, lo, hi, shift, 0};
-            issue(finer);
-            histogram(finer, false);
-            prefixes(1);
-            level = 1;
-            // prefixes of this level count from the bucket's beginning
-            b = find_bucket(1, by_count, by_count ? amount - count : amount - mass);
-            mass += s.found_mass;
-            count += s.found_count;
-            const uint32_t start = lo + (uint32_t(b) << shift);
-            hi = min(hi, lo + (uint32_t(b + 1) << shift));
-            lo = start;
-            __syncthreads();
-        }
-    };
-
-    uint64_t W = total;
-    uint64_t u = fraction32(a.uniform[row]);
-    if (u > 0xffffffffull) u = 0xffffffffull;
-    uint64_t least = ~0ull;
-    if (mp > 0.f) {
-        least = 0;
-        for (int r = 0; r < slices; ++r) least += s.min_mass[r];
-    }
-    // The head of the order in one list, where all that is asked lies in it.
-    {
-        const bool counted = top_k > 0 && uint32_t(top_k) < positive;
-        const uint64_t need = counted ? uint64_t(top_k) - 1
-                              : p < 1.f ? scaled_mass(total, fraction32(p))
-                                        : scaled_mass(least < total ? least : total, u);
-        const int b = find_bucket(0, counted, need);
-        const uint32_t tokens = b + 1 < kBuckets ? s.tokens[0][b + 1] : positive;
-        __syncthreads();
-        if (tokens <= uint32_t(kList)) {
-            const SampleCommand c{kCollect, 0, first_lo + (uint32_t(b + 1) << kFirstShift), 0, 0};
-            issue(c);
-            collect(c);
-            // tokens without mass may share the last bucket
-            head_count = int(s.listed);
-            head = head_count <= kList;
-            if (head) block_sort<NT>(s.list, head_count);
         }
     }
-    if (top_k > 0 && uint32_t(top_k) < positive) W = cross(true, uint64_t(top_k) - 1).prefix;
-    if (p < 1.f) {
-        uint64_t need = scaled_mass(W, fraction32(p));
-        if (need < 1) need = 1;
-        W = cross(false, need - 1).prefix;
-    }
-    if (least < W) W = least;
-    const Place at = cross(false, scaled_mass(W, u));
-    const SampleCommand end{at.index < 0 ? kNth : kDone, at.key, at.key + 1, 0, at.nth};
-    issue(end);
-    if (at.index < 0) nth_token(end);
-    if (tid == 0) {
-        if (at.index >= 0) a.tokens[row] = at.index;
-        if (a.log_probs)
-            a.log_probs[row] = greedy ? 0.f : -__uint_as_float(at.key) - logf(float(W) * (1.f / 2147483648.f));
-    }
-    if (many) tc::cluster_sync();
+    if (many) tc::cluster_sync();  // no CTA leaves while another may read it
 }
 
 template <class T, int NT>
 void launch_sample(hx_runtime* rt, const SampleArgs& a, uint32_t rows, long chunks, int slices)
 {
-    constexpr int EPV = Chunk<T>::EPV;
-    const int held = int((chunks + slices - 1) / slices) * EPV;
-    const size_t smem = ((sizeof(SampleShared) + 15) & ~size_t(15)) + size_t(held) * 4;
+    const size_t smem = ((sizeof(SampleShared) + 15) & ~size_t(15)) + size_t((chunks + slices - 1) / slices) * 16;
     require(uint64_t(rows) * slices <= 0x7fffffffu, HX_ERR_UNSUPPORTED, "sampling: too many rows for one call");
     auto kernel = sample_kernel<T, NT>;
     static thread_local int opted[64] = {};
@@ -563,7 +691,7 @@ void launch_sample(hx_runtime* rt, const SampleArgs& a, uint32_t rows, long chun
         HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         opted[rt->device & 63] = 1;
     }
-    launch_rows(kernel, rows * unsigned(slices), NT, slices, true, smem, rt->stream, a, slices, held);
+    launch_rows(kernel, rows * unsigned(slices), NT, slices, true, smem, rt->stream, a, slices, __builtin_ctz(unsigned(slices)));
     HX_LAUNCHED(rt);
 }
 
@@ -572,11 +700,13 @@ void launch_sample(hx_runtime* rt, const SampleArgs& a, uint32_t rows)
 {
     constexpr int EPV = Chunk<T>::EPV;
     const long chunks = row_chunks(a.logits, a.stride, rows, a.vocab, sizeof(T));
-    if (chunks * EPV <= 4096 + 2 * EPV) {
+    if (chunks <= 4096 / EPV + 1) {
         launch_sample<T, 128>(rt, a, rows, chunks, 1);
     } else {
+        // slices of 64 KB, so that two blocks share an SM; more of them, down to
+        // 4096 tokens, while the rows alone would leave SMs idle
         int s = 1;
-        while (chunks * EPV > 16640L * s) s *= 2;
+        while (chunks > 4160L * s) s *= 2;
         while (s < 8 && long(rows) * s * 2 <= rt->sm_count && chunks * EPV / (2 * s) >= 4096) s *= 2;
         launch_sample<T, 512>(rt, a, rows, chunks, s);
     }
