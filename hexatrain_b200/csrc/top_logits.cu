@@ -88,14 +88,56 @@ __device__ __forceinline__ void write_entry(const TopArgs& a, size_t row, int ra
     a.indices[row * a.k + rank] = int32_t(uint32_t(entry));
 }
 
+// One warp's exact list of the `want` first entries of elements [e0, e1) of a row,
+// unsorted, where the collection above `bound` did not serve: too many equal
+// logits, or NaN.  The list has room for them.
+template <class T>
+__device__ __noinline__ int exact_list(const T* row, int e0, int e1, float bound, int want, uint64_t* list) {
+    const int lane = threadIdx.x & 31;
+    auto key_at = [&](int i) { return descending_key(to_float(row[i])); };
+    auto count_to = [&](uint32_t t) {
+        int c = 0;
+        for (int i = e0 + lane; i < e1; i += 32) c += key_at(i) <= t;
+        return __reduce_add_sync(0xffffffffu, c);
+    };
+    // the bound is often the k-th itself
+    uint32_t t = descending_key(bound);
+    if (!(t > 0 && count_to(t - 1) < want && count_to(t) >= want)) {
+        uint32_t lo = 0, hi = 0xffffffffu;
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (count_to(mid) >= want) hi = mid; else lo = mid + 1;
+        }
+        t = lo;
+    }
+    int have = 0;
+    auto append = [&](bool equal) {
+        for (int i0 = e0; i0 < e1 && have < want; i0 += 32) {
+            const int i = i0 + lane;
+            const uint32_t key = i < e1 ? key_at(i) : 0u;
+            const bool in = i < e1 && (equal ? key == t : key < t);
+            const unsigned votes = __ballot_sync(0xffffffffu, in);
+            const int at = have + __popc(votes & ((1u << lane) - 1));
+            if (in && at < want) list[at] = entry_of(key, i);
+            have += __popc(votes);
+        }
+    };
+    append(false);
+    append(true);
+    __syncwarp();
+    return want;
+}
+
 // ---- short rows: a warp per row ---------------------------------------------------
 // Rows of up to 1024 logits (with the lead): 32 to a lane, in registers, read from
 // the second of two buffers while the next row's copy is in flight.  Bound by the
 // instructions of the selection (about 900 per row) as much as by memory.
-constexpr int kTopTeams = 4, kTopList = 512;
+constexpr int kTopTeams = 4;
+// Entries that a warp's list holds.
+__host__ __device__ constexpr int top_list(int k) { return k <= 32 ? 128 : k <= 96 ? 256 : 512; }
 
 template <class T>
-__global__ void __launch_bounds__(32 * kTopTeams)
+__global__ void __launch_bounds__(32 * kTopTeams, 6)
 top_warp_kernel(const TopArgs a, uint32_t rows)
 {
     HX_PDL_PROLOGUE();
@@ -105,7 +147,7 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
     __shared__ int s_aborted;
     const int k = int(a.k), V = int(a.vocab), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     T* rows_at = reinterpret_cast<T*>(smem + warp * (2 * kChunks * 16));
-    uint64_t* list = reinterpret_cast<uint64_t*>(smem + kTopTeams * 2 * kChunks * 16) + warp * kTopList;
+    uint64_t* list = reinterpret_cast<uint64_t*>(smem + kTopTeams * 2 * kChunks * 16) + warp * top_list(k);
     uint64_t* full = s_full + warp * 2;
     const WaitState ws{a.err, &s_aborted};
     if (threadIdx.x == 0) s_aborted = 0;
@@ -150,99 +192,87 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
         __syncwarp();
         if (row + teams < rows) px = partial_value(span_of(row + teams));
         // lane's chunks are lane, lane + 32, ...: position (32 j + lane) EPV + r
-        uint32_t key[kPerThread];
-        float top = -INFINITY;
-        {
-            float v[kPerThread];
+        float v[kPerThread];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int p = 32 * j + lane;
-                float x[EPV];
-                Chunk<T>::unpack(reinterpret_cast<const uint4*>(l)[p], x);
+        for (int j = 0; j < N; ++j) {
+            const int p = 32 * j + lane;
+            float x[EPV];
+            Chunk<T>::unpack(reinterpret_cast<const uint4*>(l)[p], x);
 #pragma unroll
-                for (int r = 0; r < EPV; ++r) v[j * EPV + r] = p < span.last ? x[r] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < kPerThread; ++i) top = fmaxf(top, v[i]);
-            top = warp_max(top);
-            if (a.lse) {
-                const float ref = fabsf(top) < INFINITY ? top : 0.f, o = ref * c;
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < kPerThread; ++i) s[i & 3] += tc::exp2_approx(fmaf(v[i], c, -o));
-                const float sum = warp_reduce((s[0] + s[1]) + (s[2] + s[3]), SumOp());
-                if (lane == 0)
-                    a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, c, -o));
-            }
-            // the keys; positions outside the row come after everything
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-#pragma unroll
-                for (int r = 0; r < EPV; ++r) {
-                    const int i = (32 * j + lane) * EPV + r - span.lead;
-                    key[j * EPV + r] = i >= 0 && i < V ? descending_key(v[j * EPV + r]) : 0xffffffffu;
-                }
+            for (int r = 0; r < EPV; ++r) v[j * EPV + r] = x[r];
         }
-        uint32_t t;
-        if (k <= 96) {  // over the 256 maxima of four logits each
-            uint32_t group[kPerThread / 4];
+        if (span.last < kChunks) {
 #pragma unroll
-            for (int i = 0; i < kPerThread / 4; ++i)
-                group[i] = min(min(key[4 * i], key[4 * i + 1]), min(key[4 * i + 2], key[4 * i + 3]));
-            t = warp_kth(group, k, 4);
+            for (int i = 0; i < kPerThread; ++i)
+                if (32 * (i / EPV) + lane >= span.last) v[i] = -INFINITY;
+        }
+        float group[kPerThread / 4], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPerThread / 4; ++i) {
+            group[i] = fmaxf(fmaxf(v[4 * i], v[4 * i + 1]), fmaxf(v[4 * i + 2], v[4 * i + 3]));
+            top = fmaxf(top, group[i]);
+        }
+        top = warp_max(top);
+        if (a.lse) {
+            const float ref = fabsf(top) < INFINITY ? top : 0.f, o = ref * c;
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) s[i & 3] += tc::exp2_approx(fmaf(v[i], c, -o));
+            const float sum = warp_reduce((s[0] + s[1]) + (s[2] + s[3]), SumOp());
+            if (lane == 0) a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, c, -o));
+        }
+        float bound;  // at least k logits reach it, and not many more
+        if (k <= 32) {  // the k-th of the 128 maxima of eight logits each
+            uint32_t key[kPerThread / 8];
+#pragma unroll
+            for (int i = 0; i < kPerThread / 8; ++i) key[i] = descending_key(fmaxf(group[2 * i], group[2 * i + 1]));
+            bound = from_descending_key(warp_kth(key, k, 4));
+        } else if (k <= 96) {  // of the 256 maxima of four
+            uint32_t key[kPerThread / 4];
+#pragma unroll
+            for (int i = 0; i < kPerThread / 4; ++i) key[i] = descending_key(group[i]);
+            bound = from_descending_key(warp_kth(key, k, 4));
         } else {
-            t = warp_kth(key, k, 64);
+            uint32_t key[kPerThread];
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) key[i] = descending_key(v[i]);
+            bound = from_descending_key(warp_kth(key, k, 64));
         }
         uint32_t mask = 0;
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) mask |= uint32_t(key[i] <= t) << i;
+        for (int i = 0; i < kPerThread; ++i) mask |= uint32_t(v[i] >= bound) << i;
         int mine = __popc(mask), count = __reduce_add_sync(0xffffffffu, mine);
-        int equals = 0;  // of those with key t, how many are wanted, in index order; 0: all
-        if (count > 384) {
-            // many equal keys: the k-th exactly, all below it and the first equal to it
-            t = warp_kth(key, k, -1);
-            mask = 0;
-#pragma unroll
-            for (int i = 0; i < kPerThread; ++i) mask |= uint32_t(key[i] < t) << i;
-            mine = __popc(mask);
-            count = __reduce_add_sync(0xffffffffu, mine);
-            equals = k - count;
+        bool listed = false;
+        if (!(bound > -INFINITY) || count > min(top_list(k), 384)) {
+            // NaN, or many equal logits
+            count = exact_list(l + span.lead, 0, V, bound, k, list);
+            listed = true;
         }
-        auto index_of = [&](int i) { return (32 * (i / EPV) + lane) * EPV + i % EPV - span.lead; };
-        int at = mine;
+        // first the places, lane 32 + bit, then each lane the entries of its share
+        uint32_t* places = reinterpret_cast<uint32_t*>(list);
+        if (!listed) {
+            int at = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, at, o);
-            if (lane >= o) at += y;
-        }
-        at -= mine;
-        for (; mask; mask &= mask - 1) {
-            const int i = index_of(__ffs(mask) - 1);
-            list[at++] = entry_of(descending_key(to_float(l[i + span.lead])), i);
-        }
-        if (equals > 0) {
-            int before = 0;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                uint32_t eq = 0;
-#pragma unroll
-                for (int r = 0; r < EPV; ++r) {
-                    const int i = (32 * j + lane) * EPV + r - span.lead;
-                    eq |= uint32_t(key[j * EPV + r] == t && i >= 0 && i < V) << r;
-                }
-                int pre = __popc(eq);
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, pre, o);
-                    if (lane >= o) pre += y;
-                }
-                const int all = __shfl_sync(0xffffffffu, pre, 31);
-                int nth = before + pre - __popc(eq);
-                for (; eq && nth < equals; eq &= eq - 1, ++nth)
-                    list[count + nth] = entry_of(t, (32 * j + lane) * EPV + __ffs(eq) - 1 - span.lead);
-                before += all;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, at, o);
+                if (lane >= o) at += y;
             }
-            count = k;
+            at -= mine;
+            for (; mask; mask &= mask - 1) places[at++] = uint32_t(lane * 32 + __ffs(mask) - 1);
+            __syncwarp();
+            // from the end, so that an entry overwrites places already read
+            for (int j0 = (count - 1) & ~31; j0 >= 0; j0 -= 32) {
+                const int j = j0 + lane;
+                uint64_t e = 0;
+                if (j < count) {
+                    const int bit = places[j] & 31, from = places[j] >> 5;
+                    const int p = (32 * (bit / EPV) + from) * EPV + bit % EPV;
+                    e = entry_of(descending_key(to_float(l[p])), p - span.lead);
+                }
+                __syncwarp();
+                if (j < count) list[j] = e;
+                __syncwarp();
+            }
         }
         __syncwarp();
         if (row + 2 * size_t(teams) < rows) {  // the row is in registers and in the list
@@ -278,11 +308,15 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
 // warps do what belongs to a row, R rows ahead and behind.  The consumers add
 // the exponentials and keep the maxima of 512 groups of one row, then go back to the row
 // before, still in the ring, for the logits that reach its bound.  The row's warp
-// finds the bound (in a cluster the largest of the CTAs' bounds), sorts what was
-// collected, and the first CTA's warp merges the CTAs' lists.  Memory bound.
-constexpr int kGroups = 512, kCollect = 512, kTopRing = 64;
+// finds the bound (in a cluster one for all CTAs), sorts what was collected, and one
+// CTA's warp, in turn, merges the CTAs' lists.  Memory bound.
+constexpr int kGroups = 512, kTopRing = 64;
 __host__ __device__ constexpr int top_blocks(int nt) { return nt == 128 ? 4 : nt == 256 ? 2 : 1; }
-__host__ __device__ constexpr int top_row_warps(int nt) { return nt == 128 ? 2 : 4; }
+__host__ __device__ constexpr int top_row_warps(int nt) { return nt == 128 ? 4 : nt == 256 ? 6 : 8; }
+
+// Entries of a row's list (a power of two): the bound lets a quarter more than k pass,
+// nearly twice as many where k is half of the groups.
+__host__ __device__ constexpr int stream_list(int k) { return k <= 64 ? 128 : k <= 128 ? 256 : 512; }
 
 struct TopShape {
     int ring, slices, log_slices, row_warps;
@@ -293,14 +327,13 @@ struct TopPost {
 template <int NT, int kSlot>
 struct TopMemory {
     size_t bars, part, groups, slots, posts, counts, lists, merge, bytes;
-    // merged: entries of all CTAs' lists together
-    __host__ __device__ TopMemory(int ring, int R, int merged) {
+    __host__ __device__ TopMemory(int ring, int R, int k, int slices) {
         size_t at = size_t(ring) * kSlot * 16;
         bars = at; at += size_t(2 * ring + 6 * R) * 8;
         at = (at + 15) & ~size_t(15);
         slots = at; at += size_t(R) * 2 * 16 * 16;
-        lists = at; at += size_t(R) * kCollect * 8;
-        merge = at; at += size_t(R) * merged * 8;
+        lists = at; at += size_t(R) * stream_list(k) * 8;
+        merge = at; at += slices > 1 ? size_t(R) * slices * ((k + 1) & ~1) * 8 : 0;
         groups = at; at += size_t(R) * kGroups * 4;
         part = at; at += size_t(R) * (NT / 32) * 4;
         posts = at; at += size_t(R) * 8;
@@ -333,46 +366,6 @@ __device__ __forceinline__ void group_max(float (&g)[4], const uint4& raw, __hal
     g[3] = fmaxf(g[3], __high2float(y));
 }
 
-// One warp's exact list of the `want` first entries of elements [e0, e1) of a row,
-// unsorted, where the collection above `bound` did not serve: too many equal
-// logits, or NaN.  The list has room for kCollect.
-template <class T>
-__device__ __noinline__ int exact_list(const T* row, int e0, int e1, float bound, int want, uint64_t* list) {
-    const int lane = threadIdx.x & 31;
-    auto key_at = [&](int i) { return descending_key(to_float(row[i])); };
-    auto count_to = [&](uint32_t t) {
-        int c = 0;
-        for (int i = e0 + lane; i < e1; i += 32) c += key_at(i) <= t;
-        return __reduce_add_sync(0xffffffffu, c);
-    };
-    // the bound is often the k-th itself
-    uint32_t t = descending_key(bound);
-    if (!(t > 0 && count_to(t - 1) < want && count_to(t) >= want)) {
-        uint32_t lo = 0, hi = 0xffffffffu;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (count_to(mid) >= want) hi = mid; else lo = mid + 1;
-        }
-        t = lo;
-    }
-    int have = 0;
-    auto append = [&](bool equal) {
-        for (int i0 = e0; i0 < e1 && have < want; i0 += 32) {
-            const int i = i0 + lane;
-            const uint32_t key = i < e1 ? key_at(i) : 0u;
-            const bool in = i < e1 && (equal ? key == t : key < t);
-            const unsigned votes = __ballot_sync(0xffffffffu, in);
-            const int at = have + __popc(votes & ((1u << lane) - 1));
-            if (in && at < want) list[at] = entry_of(key, i);
-            have += __popc(votes);
-        }
-    };
-    append(false);
-    append(true);
-    __syncwarp();
-    return want;
-}
-
 template <class T, int NT>
 __global__ void __launch_bounds__(NT + 32 + 32 * top_row_warps(NT), top_blocks(NT))
 top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
@@ -382,7 +375,8 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_aborted;
     const int k = int(a.k), V = int(a.vocab), ring = shape.ring, slices = shape.slices, R = shape.row_warps;
-    const TopMemory<NT, kSlot> mem(ring, R, slices > 1 ? slices * ((k + 1) & ~1) : 0);
+    const TopMemory<NT, kSlot> mem(ring, R, k, slices);
+    const int room = stream_list(k);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + mem.bars);
     uint64_t* empty = full + ring;
     uint64_t *formed = empty + ring, *summed = formed + R, *bounded = summed + R, *collected = bounded + R;
@@ -424,12 +418,13 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
         // ---- the rows' warps ----
         const int b = warp - NW - 1;
         float4* slots = reinterpret_cast<float4*>(smem + mem.slots) + b * 32;
-        uint64_t* list = lists + b * kCollect;
+        uint64_t* list = lists + b * room;
         const int half = (k + 1) & ~1;
         uint64_t* merge = reinterpret_cast<uint64_t*>(smem + mem.merge) + size_t(b) * slices * half;
         const float c = kLog2e / a.tau, inv_tau = 1.f / a.tau;
         unsigned exchanges = 0;
-        uint32_t phase = 0;
+        uint32_t phase = 0, merges = 0;
+        int merger = 0;  // the CTA that merges, in turn
         auto exchange = [&](float4 x) {
             const int xb = exchanges & 1;
             if (lane == 0) tc::mbar_arrive_expect_tx(joined + b, 16u * slices);
@@ -438,14 +433,20 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 store_async(tc::cluster_addr(slots + xb * 16 + rank, lane), x, tc::cluster_addr(joined + b, lane));
             stream_wait(joined + b, xb, ws);
             ++exchanges;
-            return lane < slices ? slots[xb * 16 + lane] : make_float4(0.f, -INFINITY, -INFINITY, 0.f);
+            return lane < slices ? slots[xb * 16 + lane] : make_float4(0.f, -INFINITY, -INFINITY, -INFINITY);
         };
+        // a logit to take the exponentials against: the largest of 32, loaded a row
+        // ahead (a load waits long behind the rows' copies)
+        auto sample_of = [&](size_t row) {
+            return row < rows ? to_float(static_cast<const T*>(a.logits)[row * a.stride + size_t(lane) * V / 32]) : 0.f;
+        };
+        float sample = b < R ? sample_of(team + b * teams) : 0.f;
         if (b < R)
             for (size_t row = team + b * teams; row < rows; row += R * teams, phase ^= 1) {
                 const Span<T> span = span_of(row);
                 const int e0 = max(0, span.first * EPV - span.lead), e1 = min(V, span.last * EPV - span.lead);
-                // a logit to take the exponentials against: the largest of 32
-                float ref = warp_max(to_float(span.row[size_t(lane) * V / 32]));
+                float ref = warp_max(sample);
+                sample = sample_of(row + R * teams);
                 if (!(fabsf(ref) < INFINITY)) ref = 0.f;
                 float o = ref * c;
                 if (lane == 0) {
@@ -466,12 +467,19 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 }
                 top = warp_max(top);
                 float bound = from_descending_key(warp_kth(key, k, k / 8));
+                // in a cluster also: k / slices logits of every CTA reach the smallest
+                // of these
+                float shared_bound = -INFINITY;
+                if (slices > 1) {
+                    const int share = (k + slices - 1) >> shape.log_slices;
+                    shared_bound = from_descending_key(warp_kth(key, share, share / 8));
+                }
                 float sum = warp_reduce(lane < NW ? part[b * NW + lane] : 0.f, SumOp());
                 if (slices > 1) {
-                    const float4 x = exchange(make_float4(sum, top, bound, 0.f));
+                    const float4 x = exchange(make_float4(sum, top, bound, -shared_bound));
                     sum = warp_reduce(x.x, SumOp());
                     top = warp_max(x.y);
-                    bound = warp_max(x.z);
+                    bound = fmaxf(warp_max(x.z), -warp_max(x.w));
                 }
                 if (lane == 0) {
                     posts[b].bound = bound;
@@ -496,7 +504,7 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 const int want = min(k, max(0, e1 - e0));
                 // in a cluster the bound may pass a CTA's own k-th: fewer are enough there,
                 // unless NaN leaves the row short
-                if (n > kCollect || (n < want && !(bound > -INFINITY)))
+                if (n > room || (n < want && !(bound > -INFINITY)))
                     n = exact_list(span.row, e0, e1, bound, want, list);
                 if (slices == 1) {
                     warp_sort_list(list, n);
@@ -505,34 +513,40 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 } else {
                     warp_sort_list(list, n);
                     const int give = min(n, k);
-                    if (rank == 0 && lane == 0) tc::mbar_arrive_expect_tx(merged + b, uint32_t(slices) * half * 8);
+                    if (rank == merger && lane == 0) tc::mbar_arrive_expect_tx(merged + b, uint32_t(slices) * half * 8);
                     __syncwarp();
                     for (int i = lane; i < half / 2; i += 32) {
                         const uint64_t x = 2 * i < give ? list[2 * i] : ~0ull, y = 2 * i + 1 < give ? list[2 * i + 1] : ~0ull;
-                        store_async(tc::cluster_addr(merge + rank * half + 2 * i, 0),
+                        store_async(tc::cluster_addr(merge + rank * half + 2 * i, merger),
                                     make_float4(__uint_as_float(uint32_t(x)), __uint_as_float(uint32_t(x >> 32)),
                                                 __uint_as_float(uint32_t(y)), __uint_as_float(uint32_t(y >> 32))),
-                                    tc::cluster_addr(merged + b, 0));
+                                    tc::cluster_addr(merged + b, merger));
                     }
-                    if (rank == 0) {
-                        stream_wait(merged + b, phase, ws);
+                    if (rank == merger) {
+                        stream_wait(merged + b, merges & 1, ws);
+                        ++merges;
                         // an entry's rank: its place in its own list and in every other
+                        int top_step = 1;
+                        while (top_step <= half) top_step *= 2;
                         for (int i = lane; i < slices * half; i += 32) {
                             const uint64_t x = merge[i];
                             if (x == ~0ull) continue;
                             int r = 0;
-                            for (int q = 0; q < slices; ++q) {
-                                int lo = 0, hi = half;
-                                while (lo < hi) {
-                                    const int m = (lo + hi) / 2;
-                                    if (merge[q * half + m] < x) lo = m + 1; else hi = m;
-                                }
-                                r += lo;
+                            for (int q0 = 0; q0 < slices; q0 += 4) {  // four searches at a time
+                                int at[4] = {0, 0, 0, 0};
+                                for (int step = top_step / 2; step > 0; step /= 2)
+#pragma unroll
+                                    for (int q = 0; q < 4; ++q)
+                                        if (q0 + q < slices && at[q] + step <= half &&
+                                            merge[(q0 + q) * half + at[q] + step - 1] < x)
+                                            at[q] += step;
+                                r += at[0] + at[1] + at[2] + at[3];
                             }
                             if (r < k) write_entry(a, row, r, x);
                         }
                         __syncwarp();
                     }
+                    merger = (merger + 1) & (slices - 1);
                 }
             }
     } else {
@@ -601,7 +615,7 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
             const int chunks = span.chunks();
             stream_wait(bounded + gb, g_phase, ws);
             const float bound = posts[gb].bound;
-            uint64_t* list = lists + gb * kCollect;
+            uint64_t* list = lists + gb * room;
             auto take = [&](const uint4& raw, int p) {
                 float g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 group_max(g, raw, T());
@@ -613,7 +627,7 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                     const int i = (span.first + p) * EPV + r - span.lead;
                     if (!(x[r] >= bound) || i < 0 || i >= V) continue;
                     const int at = atomicAdd(counts + gb, 1);
-                    if (at < kCollect) list[at] = entry_of(descending_key(x[r]), i);
+                    if (at < room) list[at] = entry_of(descending_key(x[r]), i);
                 }
             };
             for (int p0 = 0; p0 < chunks; p0 += kSlot) {
@@ -649,19 +663,21 @@ void launch_top_stream(hx_runtime* rt, const TopArgs& a, uint32_t rows, long chu
     const int threads = NT + 32 + 32 * top_row_warps(NT);
     const size_t limit = 233472 / kPerSm - 1024 - 256;  // shared memory of a block
     auto ring_of = [&](int s, int R) {
-        const size_t fixed = TopMemory<NT, kSlot>(0, R, s > 1 ? s * ((int(a.k) + 1) & ~1) : 0).bytes + 32;
+        const size_t fixed = TopMemory<NT, kSlot>(0, R, int(a.k), s).bytes + 32;
         return fixed < limit ? int(std::min<size_t>((limit - fixed) / (size_t(kSlot) * 16 + 16), kTopRing)) : 0;
     };
     // the ring holds two rows' slices and a slot for the copies ahead; where the
     // lists of wide records take too much, fewer rows are in flight
     auto fits = [&](int s, int R) { return 2 * int(((chunks + s - 1) / s + kSlot - 1) / kSlot) + 1 <= ring_of(s, R); };
-    int s = 1, R = top_row_warps(NT);
-    while (s < 16 && !fits(s, R)) s *= 2;
+    const int most = top_row_warps(NT), least = std::min(most, 3);
+    int s = 1;
+    while (s < 16 && !fits(s, least)) s *= 2;
+    int R = most;
     while (R > 1 && !fits(s, R)) --R;
     require(fits(s, R), HX_ERR_UNSUPPORTED, "top logits: no room for the row");
     while (NT == 512 && s < 8 && long(rows) * s * 2 <= rt->sm_count && chunks / (2 * s) >= 512 && fits(2 * s, R)) s *= 2;
     const TopShape shape{ring_of(s, R), s, __builtin_ctz(unsigned(s)), R};
-    const size_t smem = TopMemory<NT, kSlot>(shape.ring, R, s > 1 ? s * ((int(a.k) + 1) & ~1) : 0).bytes;
+    const size_t smem = TopMemory<NT, kSlot>(shape.ring, R, int(a.k), s).bytes;
     auto kernel = top_stream_kernel<T, NT>;
     static thread_local int opted[64] = {};
     if (!opted[rt->device & 63]) {
@@ -680,11 +696,11 @@ void launch_top(hx_runtime* rt, const TopArgs& a, uint32_t rows)
 {
     const long chunks = row_chunks(a.logits, a.stride, rows, a.vocab, sizeof(T));
     if (chunks <= 32 * Chunk<T>::N) {
-        const size_t smem = kTopTeams * (2 * 32 * Chunk<T>::N * 16 + kTopList * 8);
+        const size_t smem = kTopTeams * (2 * 32 * Chunk<T>::N * 16 + size_t(top_list(int(a.k))) * 8);
         auto kernel = top_warp_kernel<T>;
         static thread_local int opted[64] = {};
         if (!opted[rt->device & 63]) {
-            HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+            HX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536));
             opted[rt->device & 63] = 1;
         }
         const unsigned blocks =
