@@ -342,29 +342,51 @@ struct TopMemory {
     }
 };
 
-// The running maxima of a thread's four groups.
-__device__ __forceinline__ void group_max(float (&g)[4], const uint4& raw, float) {
-    g[0] = fmaxf(g[0], __uint_as_float(raw.x));
-    g[1] = fmaxf(g[1], __uint_as_float(raw.y));
-    g[2] = fmaxf(g[2], __uint_as_float(raw.z));
-    g[3] = fmaxf(g[3], __uint_as_float(raw.w));
-}
-__device__ __forceinline__ void group_max(float (&g)[4], const uint4& raw, __nv_bfloat16) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
-    const __nv_bfloat162 x = __hmax2(h[0], h[1]), y = __hmax2(h[2], h[3]);
-    g[0] = fmaxf(g[0], __low2float(x));
-    g[1] = fmaxf(g[1], __high2float(x));
-    g[2] = fmaxf(g[2], __low2float(y));
-    g[3] = fmaxf(g[3], __high2float(y));
-}
-__device__ __forceinline__ void group_max(float (&g)[4], const uint4& raw, __half) {
-    const __half2* h = reinterpret_cast<const __half2*>(&raw);
-    const __half2 x = __hmax2(h[0], h[1]), y = __hmax2(h[2], h[3]);
-    g[0] = fmaxf(g[0], __low2float(x));
-    g[1] = fmaxf(g[1], __high2float(x));
-    g[2] = fmaxf(g[2], __low2float(y));
-    g[3] = fmaxf(g[3], __high2float(y));
-}
+// The running maxima of a thread's four groups (16-bit types two to a register),
+// and the largest element of one chunk.
+template <class T>
+struct GroupMax;
+template <>
+struct GroupMax<float> {
+    float g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    __device__ __forceinline__ void add(const uint4& raw) {
+        g[0] = fmaxf(g[0], __uint_as_float(raw.x));
+        g[1] = fmaxf(g[1], __uint_as_float(raw.y));
+        g[2] = fmaxf(g[2], __uint_as_float(raw.z));
+        g[3] = fmaxf(g[3], __uint_as_float(raw.w));
+    }
+    __device__ __forceinline__ float of(int i) const { return g[i]; }
+    static __device__ __forceinline__ float of_chunk(const uint4& raw) {
+        return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)),
+                     fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+    }
+};
+template <class H2>
+struct GroupMax16 {
+    H2 a, b;
+    __device__ __forceinline__ void add(const uint4& raw) {
+        const H2* h = reinterpret_cast<const H2*>(&raw);
+        a = __hmax2(a, __hmax2(h[0], h[1]));
+        b = __hmax2(b, __hmax2(h[2], h[3]));
+    }
+    __device__ __forceinline__ float of(int i) const {
+        const H2 x = i < 2 ? a : b;
+        return i & 1 ? __high2float(x) : __low2float(x);
+    }
+    static __device__ __forceinline__ float of_chunk(const uint4& raw) {
+        const H2* h = reinterpret_cast<const H2*>(&raw);
+        const H2 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(x), __high2float(x));
+    }
+};
+template <>
+struct GroupMax<__nv_bfloat16> : GroupMax16<__nv_bfloat162> {
+    __device__ __forceinline__ GroupMax() { a = b = __float2bfloat162_rn(-INFINITY); }
+};
+template <>
+struct GroupMax<__half> : GroupMax16<__half2> {
+    __device__ __forceinline__ GroupMax() { a = b = __float2half2_rn(-INFINITY); }
+};
 
 template <class T, int NT>
 __global__ void __launch_bounds__(NT + 32 + 32 * top_row_warps(NT), top_blocks(NT))
@@ -504,8 +526,15 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 const int want = min(k, max(0, e1 - e0));
                 // in a cluster the bound may pass a CTA's own k-th: fewer are enough there,
                 // unless NaN leaves the row short
-                if (n > room || (n < want && !(bound > -INFINITY)))
+                if (n > room || (n < want && !(bound > -INFINITY))) {
                     n = exact_list(span.row, e0, e1, bound, want, list);
+                } else {
+                    for (int i = lane; i < n; i += 32) {
+                        const int at = int(uint32_t(list[i]));
+                        list[i] = entry_of(descending_key(to_float(span.row[at])), at);
+                    }
+                    __syncwarp();
+                }
                 if (slices == 1) {
                     warp_sort_list(list, n);
                     for (int i = lane; i < k; i += 32) write_entry(a, row, i, list[i]);
@@ -561,9 +590,10 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
             const int chunks = span_of(row).chunks();
             stream_wait(formed + sb, s_phase, ws);
             const float o = posts[sb].o;
-            float sum = 0.f, g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float sum = 0.f;
+            GroupMax<T> g;
             auto add = [&](const uint4& raw) {
-                group_max(g, raw, T());
+                g.add(raw);
                 if (sums) {
                     float e[EPV];
                     Chunk<T>::unpack(raw, e);
@@ -594,13 +624,13 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
             }
             float* to = groups + sb * kGroups;
             if (NT == 512) {
-                to[tid] = fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3]));
+                to[tid] = fmaxf(fmaxf(g.of(0), g.of(1)), fmaxf(g.of(2), g.of(3)));
             } else if (NT == 256) {
-                to[tid] = fmaxf(g[0], g[1]);
-                to[tid + 256] = fmaxf(g[2], g[3]);
+                to[tid] = fmaxf(g.of(0), g.of(1));
+                to[tid + 256] = fmaxf(g.of(2), g.of(3));
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) to[tid + 128 * i] = g[i];
+                for (int i = 0; i < 4; ++i) to[tid + 128 * i] = g.of(i);
             }
             if (sums) sum = warp_reduce(sum, SumOp());
             __syncwarp();
@@ -616,18 +646,20 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
             stream_wait(bounded + gb, g_phase, ws);
             const float bound = posts[gb].bound;
             uint64_t* list = lists + gb * room;
+            // (not unrolled: few chunks hold one, and each thread few)
             auto take = [&](const uint4& raw, int p) {
-                float g[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                group_max(g, raw, T());
-                if (!(fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])) >= bound)) return;
                 float x[EPV];
                 Chunk<T>::unpack(raw, x);
+                uint32_t mask = 0;
 #pragma unroll
-                for (int r = 0; r < EPV; ++r) {
-                    const int i = (span.first + p) * EPV + r - span.lead;
-                    if (!(x[r] >= bound) || i < 0 || i >= V) continue;
+                for (int r = 0; r < EPV; ++r) mask |= uint32_t(x[r] >= bound) << r;
+#pragma unroll 1
+                for (; mask; mask &= mask - 1) {
+                    const int i = (span.first + p) * EPV + __ffs(mask) - 1 - span.lead;
+                    if (i < 0 || i >= V) continue;
                     const int at = atomicAdd(counts + gb, 1);
-                    if (at < room) list[at] = entry_of(descending_key(x[r]), i);
+                    if (at >= room) break;
+                    list[at] = uint32_t(i);  // the row's warp adds the key
                 }
             };
             for (int p0 = 0; p0 < chunks; p0 += kSlot) {
@@ -637,9 +669,13 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 for (int q = 0; q < U; ++q) raw[q] = from[q * NT];
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(empty + back_at.slot);
+                uint32_t holds = 0;
 #pragma unroll
                 for (int q = 0; q < U; ++q)
-                    if (p0 + q * NT + tid < chunks) take(raw[q], p0 + q * NT + tid);
+                    holds |= uint32_t(p0 + q * NT + tid < chunks && GroupMax<T>::of_chunk(raw[q]) >= bound) << q;
+#pragma unroll
+                for (int q = 0; q < U; ++q)
+                    if (holds >> q & 1u) take(raw[q], p0 + q * NT + tid);
                 back_at.next(ring);
             }
             __syncwarp();
