@@ -18,9 +18,10 @@
 // 1/T: the first largest logit, log-probability 0.  A row whose logits are all
 // -inf gets token -1 and -inf; one with a NaN or +inf gets -1 and NaN.
 //
-// No row is sorted.  y >= 0, so its bits order it: a histogram of counts and
-// masses over the bits (64 buckets to an octave) finds the bucket in which a
-// prefix crosses an amount; the bucket's few tokens are collected and sorted.
+// No row is sorted: a histogram of masses (and counts, for top-k) over y finds the
+// bucket in which a prefix crosses an amount, and the bucket's few tokens are
+// collected and sorted; a bucket with too many gets a histogram of its own, over
+// the bits of y, which order it.
 #include <cmath>
 
 #include "head_rows.cuh"
@@ -72,46 +73,56 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t addr, uint32_t x) {
     return old;
 }
 
-constexpr int kBuckets = 512;
-constexpr uint32_t kHeadKey = 0x41000000u;    // bits of 8.0: the first histogram's end
-constexpr uint32_t kTopKey = 0x42000000u;     // bits of 32.0: above it no token has mass
-constexpr int kFirstShift = 17;               // 64 buckets to an octave, from 1/32
-constexpr uint32_t kFirstKey = kHeadKey - (uint32_t(kBuckets) << kFirstShift);
+constexpr float kNoMass = 24.f;               // tokens beyond have no mass: exp(-24) < 2^-31
+constexpr uint32_t kNoMassKey = 0x41c00000u;  // the bits of 24.0
+constexpr int kFine = 512;                    // buckets of a bucket's own histogram
 constexpr int kList = 128;                    // tokens that are collected and sorted at once
-constexpr int kPerLane = kBuckets / 32;
+// Buckets of the row's histogram, equal steps of y: few tokens in each, and few
+// threads of a warp in the same.
+__host__ __device__ constexpr int coarse_buckets(int nt) { return nt == 128 ? 512 : 2048; }
 
 // A pass over the row, asked for by the first warp of the first CTA.
-enum SampleStep { kDone = 0, kHistogram, kCollect, kNth };
+enum SampleStep { kDone = 0, kCoarse, kFineStep, kCollect, kNth };
 struct SampleCommand {
     int step;
-    uint32_t lo, hi;    // keys [lo, hi)
-    uint32_t lo2, hi2;  // kCollect: and [lo2, hi2)
-    int shift;          // kHistogram: bucket = (key - lo2) >> shift, 0 below lo2
-    uint32_t nth;       // kNth: which of the tokens with key lo
-    int level, sums;    // kHistogram: where to; with the sums beyond hi
+    int b0, b1;       // of the tokens in the row's buckets [b0, b1]
+    int c0, c1;       // kCollect: and in [c0, c1]
+    uint32_t lo, hi;  // those with keys in [lo, hi)
+    int shift;        // kFineStep: bucket = (key - lo) >> shift
+    uint32_t nth;     // kNth: which of the tokens with key lo
+    int masses;       // kCoarse: masses too, not counts alone
 };
 
 // What the thinking warp keeps between passes.
 enum Goal { kTopK, kTopP, kToken };
 struct Thought {
-    int goal, pending, head_count, refine_shift;  // pending: the step whose result is awaited, -1 at first
-    bool by_count, head, planned;
-    uint64_t W, amount, mass, least, total, plan_mass;
-    uint32_t count, lo, hi, tokens;
-    uint32_t plan_hi;           // the end of the second interval, for the token that follows
+    int goal, pending, head_count, shift, bucket;  // pending: the step whose result is awaited
+    bool by_count, head, planned, masses;
+    uint64_t W, amount, mass, least, plan_mass;
+    uint32_t count, lo, hi;  // mass and tokens before [lo, hi)
+    int plan_b1;
 };
 
+// A histogram: in a slice mass = high 2^16 + low, in the first CTA then the row's
+// masses and counts.
+template <int N>
+struct Histogram {
+    uint2 parts[N];
+    uint32_t count[N];
+    uint64_t lane_mass[33];  // before a lane's buckets, and in all
+    uint32_t lane_count[33];
+    __device__ __forceinline__ uint64_t& mass(int b) { return reinterpret_cast<uint64_t*>(parts)[b]; }
+    __device__ __forceinline__ uint64_t mass(int b) const { return reinterpret_cast<const uint64_t*>(parts)[b]; }
+};
+template <int NB>
 struct SampleShared {
-    uint32_t low[kBuckets], high[kBuckets], count[kBuckets];  // this slice's: mass = high 2^16 + low
-    uint64_t mass[2][kBuckets];                               // the row's, of the first histogram and the last
-    uint32_t tokens[2][kBuckets];
-    uint64_t lane_mass[2][33];                                // before a lane's buckets, and in all
-    uint32_t lane_tokens[2][33];
-    uint64_t list[kList];                                     // key 2^32 + index
+    Histogram<NB> coarse;
+    Histogram<kFine> fine;
+    uint64_t list[kList];  // key 2^32 + index
     uint64_t scan[32];
     float maxima[16];
-    uint64_t rest_mass[16], min_mass[16];                     // beyond the first histogram; within min-p's limit
-    uint32_t rest_tokens[16], nth_counts[16];
+    uint64_t min_mass[16];  // within min-p's limit
+    uint32_t nth_counts[16];
     uint32_t listed;
     SampleCommand command;
     Thought thought;
@@ -154,11 +165,11 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t x) {
 // the instruction cache has to bring in for every row.
 
 // One warp sorts the first c <= kList entries of the list.
-__device__ __noinline__ void sort_list(SampleShared& s, int c) {
+__device__ __noinline__ void sort_list(uint64_t* list, int c) {
     const int lane = threadIdx.x & 31;
     int size = 32;
     while (size < c) size *= 2;
-    for (int i = c + lane; i < size; i += 32) s.list[i] = ~0ull;
+    for (int i = c + lane; i < size; i += 32) list[i] = ~0ull;
     __syncwarp();
 #pragma unroll 1
     for (int k = 2; k <= size; k *= 2)
@@ -167,33 +178,35 @@ __device__ __noinline__ void sort_list(SampleShared& s, int c) {
 #pragma unroll 1
             for (int t = lane; t < size / 2; t += 32) {
                 const int i = 2 * t - (t & (j - 1));
-                const uint64_t a = s.list[i], b = s.list[i + j];
+                const uint64_t a = list[i], b = list[i + j];
                 if ((a > b) == ((i & k) == 0)) {
-                    s.list[i] = b;
-                    s.list[i + j] = a;
+                    list[i] = b;
+                    list[i + j] = a;
                 }
             }
             __syncwarp();
         }
 }
-// Prefixes before each lane's 16 buckets.
-__device__ __noinline__ void lane_prefixes(SampleShared& s, int level) {
+// Prefixes before each lane's N / 32 buckets.
+template <int N>
+__device__ __noinline__ void lane_prefixes(Histogram<N>& h) {
     const int lane = threadIdx.x & 31;
+    constexpr int per = N / 32;
     uint64_t w = 0;
     uint32_t k = 0;
-    const ulonglong2* ms = reinterpret_cast<const ulonglong2*>(&s.mass[level][lane * kPerLane]);
-    const uint4* ts = reinterpret_cast<const uint4*>(&s.tokens[level][lane * kPerLane]);
-#pragma unroll
-    for (int i = 0; i < kPerLane / 2; ++i) w += ms[i].x + ms[i].y;
-#pragma unroll
-    for (int i = 0; i < kPerLane / 4; ++i) k += ts[i].x + ts[i].y + ts[i].z + ts[i].w;
+#pragma unroll 4
+    for (int i = 0; i < per; ++i) {  // (each lane from a place of its own: no bank conflicts)
+        const int b = lane * per + ((i + lane) & (per - 1));
+        w += h.mass(b);
+        k += h.count[b];
+    }
     const uint64_t ws = warp_scan(w);
     const uint32_t ks = uint32_t(warp_scan(k));
-    s.lane_mass[level][lane] = ws - w;
-    s.lane_tokens[level][lane] = ks - k;
+    h.lane_mass[lane] = ws - w;
+    h.lane_count[lane] = ks - k;
     if (lane == 31) {
-        s.lane_mass[level][32] = ws;
-        s.lane_tokens[level][32] = ks;
+        h.lane_mass[32] = ws;
+        h.lane_count[32] = ks;
     }
     __syncwarp();
 }
@@ -203,25 +216,39 @@ struct Bucket {
     uint32_t count;
 };
 // The bucket in which the prefix exceeds `want` (which lies in one).
-__device__ __noinline__ Bucket find_bucket(const SampleShared& s, int level, bool counted, uint64_t want) {
+template <int N>
+__device__ __noinline__ Bucket find_bucket(const Histogram<N>& h, bool counted, uint64_t want) {
     const int lane = threadIdx.x & 31;
-    const bool here = counted ? s.lane_tokens[level][lane] <= want && want < s.lane_tokens[level][lane + 1]
-                              : s.lane_mass[level][lane] <= want && want < s.lane_mass[level][lane + 1];
+    constexpr int per = N / 32;
+    const bool here = counted ? h.lane_count[lane] <= want && want < h.lane_count[lane + 1]
+                              : h.lane_mass[lane] <= want && want < h.lane_mass[lane + 1];
     const int src = (__ffs(__ballot_sync(0xffffffffu, here)) - 1) & 31;
-    const int b = src * kPerLane + (lane & (kPerLane - 1));
-    const uint64_t w = lane < kPerLane ? s.mass[level][b] : 0;
-    const uint32_t k = lane < kPerLane ? s.tokens[level][b] : 0;
-    const uint64_t we = s.lane_mass[level][src] + warp_scan(w);
-    const uint32_t ke = s.lane_tokens[level][src] + uint32_t(warp_scan(k));
-    const int at = (__ffs(__ballot_sync(0xffffffffu, lane < kPerLane && want < (counted ? uint64_t(ke) : we))) - 1) & 31;
-    return {src * kPerLane + at, __shfl_sync(0xffffffffu, we - w, at), __shfl_sync(0xffffffffu, ke - k, at)};
+    uint64_t before = h.lane_mass[src];
+    uint32_t tokens = h.lane_count[src];
+    Bucket r{src * per, before, tokens};
+#pragma unroll 1
+    for (int i0 = 0; i0 < per; i0 += 32) {
+        const int b = src * per + i0 + lane;
+        const bool in = i0 + lane < per;
+        const uint64_t w = in ? h.mass(b) : 0, we = before + warp_scan(w);
+        const uint32_t k = in ? h.count[b] : 0, ke = tokens + uint32_t(warp_scan(k));
+        const unsigned hit = __ballot_sync(0xffffffffu, in && want < (counted ? uint64_t(ke) : we));
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            r = {src * per + i0 + at, __shfl_sync(0xffffffffu, we - w, at), __shfl_sync(0xffffffffu, ke - k, at)};
+            break;
+        }
+        before = __shfl_sync(0xffffffffu, we, 31);
+        tokens = __shfl_sync(0xffffffffu, ke, 31);
+    }
+    return r;
 }
 struct Found {
     uint64_t entry, prefix;  // the prefix mass with the entry
 };
 // Where the prefix of the sorted list's entries [from, to) exceeds `want`, given
 // the mass and the count before them.
-__device__ __noinline__ Found find_in_list(const SampleShared& s, int from, int to, uint64_t w0, uint64_t k0, bool counted,
+__device__ __noinline__ Found find_in_list(const uint64_t* list, int from, int to, uint64_t w0, uint64_t k0, bool counted,
                                            uint64_t want) {
     const int lane = threadIdx.x & 31;
     uint64_t e = 0, prefix = 0;
@@ -229,7 +256,7 @@ __device__ __noinline__ Found find_in_list(const SampleShared& s, int from, int 
 #pragma unroll 1
     for (int j0 = from; j0 < to && !hit; j0 += 32) {
         const int j = j0 + lane;
-        e = j < to ? s.list[j] : 0;
+        e = j < to ? list[j] : 0;
         const uint32_t w = j < to ? mass_of_key(uint32_t(e >> 32)) : 0u;
         prefix = w0 + warp_scan(w);
         hit = __ballot_sync(0xffffffffu, j < to && (counted ? k0 + (j - from) == want : want < prefix && want >= prefix - w));
@@ -238,31 +265,43 @@ __device__ __noinline__ Found find_in_list(const SampleShared& s, int from, int 
     const int src = (__ffs(hit) - 1) & 31;
     return {__shfl_sync(0xffffffffu, e, src), __shfl_sync(0xffffffffu, prefix, src)};
 }
-// The first entry of the sorted list with a key >= `key`.
-__device__ __forceinline__ int list_from(const SampleShared& s, int c, uint32_t key) {
+// The mass of the sorted list's entries with y <= limit.
+__device__ __noinline__ uint64_t list_mass(const uint64_t* list, int c, float limit) {
+    uint64_t w = 0;
+#pragma unroll 1
+    for (int j = threadIdx.x & 31; j < c; j += 32) {
+        const float y = __uint_as_float(uint32_t(list[j] >> 32));
+        if (y <= limit) w += mass_of(y);
+    }
+    return warp_reduce(w, SumOp());
+}
+// Entries of the sorted list with a key < `key`.
+__device__ __noinline__ int list_below(const uint64_t* list, int c, uint32_t key) {
     int at = 0;
 #pragma unroll 1
     for (int j0 = 0; j0 < c; j0 += 32) {
         const int j = j0 + (threadIdx.x & 31);
-        at += __popc(__ballot_sync(0xffffffffu, j < c && uint32_t(s.list[j] >> 32) < key));
+        at += __popc(__ballot_sync(0xffffffffu, j < c && uint32_t(list[j] >> 32) < key));
     }
     return at;
 }
 
 // One block per row, or a cluster of them with a slice each, held in shared memory.
 // The first warp of the first CTA thinks, all others make the passes that it asks
-// for: a histogram, the collection of a bucket's tokens, rarely the nth of equal
-// tokens.  Most tokens lie far below the largest (beyond y = 8): the first pass
-// gives them no buckets, only their sum.
+// for: the row's histogram, the collection of a bucket's tokens, rarely a bucket's
+// own histogram or the nth of equal tokens.  Bound by the instructions of the passes (about
+// 25 per token in the first, which forms expf of every one) and by the latency
+// between them.  Few-token filters (top_k <= 128) need no masses but those of
+// the tokens they keep: their histogram only counts.
 template <class T, int NT>
 __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8)
 sample_kernel(const SampleArgs a, int slices, int log_slices)
 {
     HX_PDL_PROLOGUE();
+    constexpr int NB = coarse_buckets(NT), EPV = Chunk<T>::EPV;
     extern __shared__ __align__(16) uint8_t smem[];
-    SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
-    uint4* held = reinterpret_cast<uint4*>(smem + ((sizeof(SampleShared) + 15) & ~size_t(15)));
-    constexpr int EPV = Chunk<T>::EPV;
+    SampleShared<NB>& s = *reinterpret_cast<SampleShared<NB>*>(smem);
+    uint4* held = reinterpret_cast<uint4*>(smem + ((sizeof(SampleShared<NB>) + 15) & ~size_t(15)));
     const int tid = threadIdx.x, lane = tid & 31, V = int(a.vocab);
     const int rank = int(blockIdx.x) & (slices - 1);
     const size_t row = blockIdx.x >> log_slices;
@@ -283,6 +322,9 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         m = max_or_nan(m, chunk_max(raw, T()));
     };
     const float uniform = thinker ? a.uniform[row] : 0.f;
+    const float temp = a.temperature ? a.temperature[row] : 1.f;
+    const int top_k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f;
     const int whole0 = lead > 0 && first == 0 ? 1 : 0, whole1 = max(whole0, min(n, (V + lead) / EPV - first));
     const uint4* from = reinterpret_cast<const uint4*>(l - lead) + first;
     for (int c0 = whole0 + tid; c0 < whole1; c0 += 4 * NT) {
@@ -307,6 +349,10 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
             keep(c, Chunk<T>::pack(x));
         }
     }
+    for (int b = tid; b < NB; b += NT) {
+        s.coarse.parts[b] = make_uint2(0u, 0u);
+        s.coarse.count[b] = 0u;
+    }
     bool nan = __syncthreads_or(!(m < INFINITY)) != 0;
     m = block_reduce<NT>(m, reinterpret_cast<float*>(s.scan), MaxOp());
     if (many) {
@@ -327,7 +373,6 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         return;  // the whole cluster
     }
 
-    const float temp = a.temperature ? a.temperature[row] : 1.f;
     const float inv_t = __fdiv_rn(1.f, temp);
     if (!(temp > 0.f) || temp == INFINITY || inv_t == INFINITY) {  // the first largest logit
         int at = 0x7fffffff;
@@ -353,194 +398,188 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         }
         return;  // the whole cluster
     }
-    const int top_k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f;
-    const float limit = mp > 0.f ? fmaxf(-logf(mp), 0.f) : INFINITY;
-    const bool whole = top_k <= 0 || (mp > 0.f && limit > 8.f);
+    const float limit = mp > 0.f ? fmaxf(-logf(mp), 0.f) : -1.f;
+    // the row's bucket of y < kNoMass
+    constexpr float kScale = float(NB) / kNoMass;
+    auto bucket_of = [](float y) { return min(int(y * kScale), NB - 1); };
+    auto key_below = [](int b) { return b <= 1 ? 0u : __float_as_uint(float(b - 1) / kScale); };  // at most those of bucket b
+    auto key_above = [](int b) { return min(kNoMassKey, __float_as_uint(float(b + 2) / kScale)); };  // above them
 
     // Goes on until a pass over the row is needed.
     auto think = [&](bool begin) {
         Thought t;
         if (begin) {
             t = Thought{};
-            t.pending = -1;
-            t.least = ~0ull;
+            t.masses = top_k <= 0 || top_k > kList;
         } else {
             t = s.thought;
         }
-        auto ask = [&](int step, uint32_t lo, uint32_t hi, uint32_t lo2, uint32_t hi2, int shift, uint32_t nth, int sums) {
-            t.pending = sums ? -2 : step;
+        auto ask = [&](const SampleCommand& c) {
+            t.pending = c.step;
             __syncwarp();
             if (lane == 0) {
-                s.command = {step, lo, hi, lo2, hi2, shift, nth, sums ? 0 : 1, sums};
+                s.command = c;
                 s.listed = 0;
                 s.thought = t;
             }
         };
-        auto collect = [&](uint32_t lo, uint32_t hi, uint32_t lo2, uint32_t hi2) { ask(kCollect, lo, hi, lo2, hi2, 0, 0, 0); };
-        auto finer = [&] {
-            t.refine_shift = 0;
-            while (((t.hi - 1 - t.lo) >> t.refine_shift) >= uint32_t(kBuckets)) ++t.refine_shift;
-            ask(kHistogram, t.lo, t.hi, t.lo, 0, t.refine_shift, 0, 0);
+        auto collect = [&](int b0, int b1, int c0, int c1, uint32_t lo, uint32_t hi) {
+            ask({kCollect, b0, b1, c0, c1, lo, hi, 0, 0, 0});
         };
-        auto bucket_lo = [](int b) { return b == 0 ? 0u : kFirstKey + (uint32_t(b) << kFirstShift); };
-        auto bucket_hi = [](int b) { return kFirstKey + (uint32_t(b + 1) << kFirstShift); };
         const uint64_t u = min(fraction32(uniform), uint64_t(0xffffffffu)), p32 = fraction32(p);
         Found found{};
         bool have = false;  // `found` answers the goal
-        if (begin) lane_prefixes(s, 0);
-        const uint64_t head_mass = s.lane_mass[0][32];
-        const uint32_t head_tokens = s.lane_tokens[0][32];
-        if (t.pending < 0) {
-            if (begin && !whole && uint32_t(top_k) > head_tokens) {  // the first k reach beyond the first histogram
-                ask(kHistogram, 0, kHeadKey, kFirstKey, 0, kFirstShift, 0, 1);
+        if (t.pending == kCoarse || begin) {  // the row's histogram is there
+            lane_prefixes(s.coarse);
+            const uint32_t tokens = s.coarse.lane_count[32];
+            t.least = ~0ull;
+            if (!t.masses) {
+                // the first k, or all that have mass, in one list, if it holds them
+                t.amount = min(uint32_t(top_k), tokens) - 1;
+                const Bucket b = find_bucket(s.coarse, true, t.amount);
+                if (b.count + s.coarse.count[b.at] <= uint32_t(kList)) {
+                    t.head = true;
+                    t.by_count = true;
+                    t.goal = kTopK;
+                    collect(0, b.at, 1, 0, 0, key_above(b.at));
+                    return;
+                }
+                t.masses = true;
+                ask({kCoarse, 0, NB - 1, 1, 0, 0, kNoMassKey, 0, 0, 1});
                 return;
             }
-            t.total = head_mass;
-            t.tokens = head_tokens;
-            if (whole || t.pending == -2)
-                for (int r = 0; r < slices; ++r) {
-                    t.total += s.rest_mass[r];
-                    t.tokens += s.rest_tokens[r];
-                }
+            t.W = s.coarse.lane_mass[32];
             if (mp > 0.f) {
                 t.least = 0;
                 for (int r = 0; r < slices; ++r) t.least += s.min_mass[r];
             }
-            t.W = t.total;
-            const bool counted = top_k > 0 && uint32_t(top_k) <= t.tokens;
-            t.goal = counted ? kTopK : p < 1.f ? kTopP : kToken;
-            // all that will be asked lies below this: where few tokens do, they
-            // are collected once
-            const uint64_t most = counted ? uint64_t(top_k) - 1
-                                  : p < 1.f ? scaled_mass(t.total, p32) : scaled_mass(min(t.least, t.total), u);
-            if (counted ? most < head_tokens : most < head_mass) {
-                const Bucket b = find_bucket(s, 0, counted, most);
-                if (b.count + s.tokens[0][b.at] <= uint32_t(kList)) {
-                    t.head = true;
-                    collect(0, bucket_hi(b.at), 0, 0);
-                    return;
-                }
-            }
-        } else if (t.head && t.head_count == 0) {
-            t.head_count = int(s.listed);
-            sort_list(s, t.head_count);
+            t.goal = top_k > 0 && uint32_t(top_k) < tokens ? kTopK : p < 1.f ? kTopP : kToken;
+            t.pending = kDone;
         } else if (t.pending == kCollect) {
             const int c = int(s.listed);
             if (c > kList) {
                 if (t.planned) {  // together too many: one after the other
                     t.planned = false;
-                    collect(t.lo, t.hi, 0, 0);
-                } else {
-                    finer();
+                    collect(t.bucket, t.bucket, 1, 0, t.lo, t.hi);
+                    return;
                 }
+                // a histogram of this bucket
+                t.shift = 0;
+                while (((t.hi - 1 - t.lo) >> t.shift) >= uint32_t(kFine)) ++t.shift;
+                ask({kFineStep, t.bucket, t.bucket, 1, 0, t.lo, t.hi, t.shift, 0, 0});
                 return;
             }
-            sort_list(s, c);
-            const bool apart = t.planned && t.plan_hi <= t.lo;
-            const int from = apart ? list_from(s, c, t.lo) : 0;
-            found = find_in_list(s, from, c, t.mass, t.count, t.by_count, t.amount);
+            sort_list(s.list, c);
+            if (t.head) {
+                t.head_count = c;
+                if (mp > 0.f) t.least = list_mass(s.list, c, limit);
+                found = find_in_list(s.list, 0, c, 0, 0, true, t.amount);
+            } else {
+                // the token's tokens first, if they were collected too
+                const int from = t.planned && t.plan_b1 < t.bucket ? list_below(s.list, c, t.lo) : 0;
+                if (t.planned && t.plan_b1 < t.bucket) {
+                    // (lo is a lower bound of the bucket's keys: its neighbour's may reach above)
+                    int f = from;
+                    while (f < c && bucket_of(__uint_as_float(uint32_t(s.list[f] >> 32))) < t.bucket) ++f;
+                    found = find_in_list(s.list, f, c, t.mass, t.count, t.by_count, t.amount);
+                    t.W = min(found.prefix, t.least);
+                    t.goal = kToken;
+                    found = find_in_list(s.list, 0, f, t.plan_mass, 0, false, scaled_mass(t.W, u));
+                } else {
+                    found = find_in_list(s.list, 0, c, t.mass, t.count, t.by_count, t.amount);
+                    if (t.planned) {  // in one interval
+                        t.W = min(found.prefix, t.least);
+                        t.goal = kToken;
+                        found = find_in_list(s.list, 0, c, t.mass, 0, false, scaled_mass(t.W, u));
+                    }
+                }
+            }
             have = true;
-            if (t.planned) {  // the token that follows lies in the list too
-                t.W = min(found.prefix, t.least);
-                t.goal = kToken;
-                found = find_in_list(s, 0, apart ? from : c, t.plan_mass, 0, false, scaled_mass(t.W, u));
+        } else {  // a bucket's histogram
+            lane_prefixes(s.fine);
+            const Bucket b = find_bucket(s.fine, t.by_count, t.by_count ? t.amount - t.count : t.amount - t.mass);
+            t.mass += b.mass;
+            t.count += b.count;
+            t.hi = min(t.hi, t.lo + (uint32_t(b.at + 1) << t.shift));
+            t.lo += uint32_t(b.at) << t.shift;
+            if (t.hi - t.lo > 1) {
+                collect(t.bucket, t.bucket, 1, 0, t.lo, t.hi);
+                return;
+            }
+            // one key: its tokens have one mass
+            const uint64_t w = mass_of_key(t.lo), nth = t.by_count ? t.amount - t.count : (t.amount - t.mass) / w;
+            found = {uint64_t(t.lo) << 32, t.mass + (nth + 1) * w};
+            have = true;
+            if (t.goal == kToken) {
+                t.amount = nth;
+                t.pending = kNth;
             }
         }
 #pragma unroll 1
         for (;;) {
-            if (!have) {
-                if (t.pending == kHistogram) {  // continue within [lo, hi)
-                    lane_prefixes(s, 1);
-                    const Bucket b = find_bucket(s, 1, t.by_count, t.by_count ? t.amount - t.count : t.amount - t.mass);
-                    t.mass += b.mass;
-                    t.count += b.count;
-                    t.hi = min(t.hi, t.lo + (uint32_t(b.at + 1) << t.refine_shift));
-                    t.lo += uint32_t(b.at) << t.refine_shift;
-                } else {  // a new goal
-                    t.by_count = t.goal == kTopK;
-                    if (t.goal == kTopK) {
-                        t.amount = uint64_t(top_k) - 1;
-                    } else if (t.goal == kTopP) {
-                        const uint64_t need = scaled_mass(t.W, p32);
-                        t.amount = need < 1 ? 0 : need - 1;
-                    } else {
-                        t.W = min(t.W, t.least);
-                        t.amount = scaled_mass(t.W, u);
+            if (have) {  // the goal's answer
+                if (t.goal == kToken) {
+                    if (lane == 0) {
+                        if (t.pending != kNth) a.tokens[row] = int32_t(uint32_t(found.entry));
+                        if (a.log_probs)
+                            a.log_probs[row] = -__uint_as_float(uint32_t(found.entry >> 32)) -
+                                               logf(float(t.W) * (1.f / 2147483648.f));
                     }
-                    if (t.head) {
-                        found = find_in_list(s, 0, t.head_count, 0, 0, t.by_count, t.amount);
-                        have = true;
-                    } else if (t.by_count ? t.amount < head_tokens : t.amount < head_mass) {
-                        const Bucket b = find_bucket(s, 0, t.by_count, t.amount);
-                        t.lo = bucket_lo(b.at);
-                        t.hi = bucket_hi(b.at);
-                        t.mass = b.mass;
-                        t.count = b.count;
-                        t.planned = false;
-                        if (t.goal == kTopP || (t.goal == kTopK && !(p < 1.f))) {
-                            // W will lie in this bucket: but for that the token's bucket is
-                            // known, and its tokens are collected in the same pass
-                            const Bucket b1 = find_bucket(s, 0, false, scaled_mass(min(b.mass, t.least), u));
-                            const Bucket b2 = find_bucket(s, 0, false, scaled_mass(min(b.mass + s.mass[0][b.at], t.least), u));
-                            if (b2.count + s.tokens[0][b2.at] - b1.count + s.tokens[0][b.at] <= uint32_t(kList)) {
-                                t.planned = true;
-                                t.plan_mass = b1.mass;
-                                t.plan_hi = bucket_hi(b2.at);
-                                if (b2.at < b.at) {
-                                    collect(t.lo, t.hi, bucket_lo(b1.at), t.plan_hi);
-                                    return;
-                                }
-                                // one interval: the list begins at the token's first bucket
-                                t.lo = bucket_lo(b1.at);
-                                t.mass = b1.mass;
-                                t.count = b1.count;
-                            }
-                        }
-                    } else {  // beyond the first histogram
-                        t.mass = head_mass;
-                        t.count = head_tokens;
-                        t.lo = kHeadKey;
-                        t.hi = kTopKey;
-                        finer();
-                        return;
-                    }
+                    const uint32_t key = uint32_t(found.entry >> 32);
+                    ask({t.pending == kNth ? kNth : kDone, 0, NB - 1, 1, 0, key, key + 1, 0, uint32_t(t.amount), 0});
+                    return;
                 }
-                if (!have) {
-                    if (t.hi - t.lo > 1) {
-                        collect(t.lo, t.hi, 0, 0);
-                        return;
-                    }
-                    // one key: its tokens have one mass
-                    const uint64_t w = mass_of_key(t.lo);
-                    const uint64_t nth = t.by_count ? t.amount - t.count : (t.amount - t.mass) / w;
-                    found.prefix = t.mass + (nth + 1) * w;
-                    if (t.goal == kToken) {
-                        found.entry = uint64_t(t.lo) << 32;
-                        t.amount = nth;
-                    }
-                }
+                t.W = found.prefix;
+                t.goal = t.goal == kTopK && p < 1.f ? kTopP : kToken;
+                have = false;
             }
-            if (t.goal == kToken) {
-                if (lane == 0) {
-                    if (have) a.tokens[row] = int32_t(uint32_t(found.entry));
-                    if (a.log_probs)
-                        a.log_probs[row] = -__uint_as_float(uint32_t(found.entry >> 32)) -
-                                           logf(float(t.W) * (1.f / 2147483648.f));
-                }
-                ask(have ? kDone : kNth, t.lo, t.lo + 1, 0, 0, 0, uint32_t(t.amount), 0);
+            // the next goal
+            t.by_count = t.goal == kTopK;
+            if (t.goal == kTopK) {
+                t.amount = uint64_t(top_k) - 1;
+            } else if (t.goal == kTopP) {
+                const uint64_t need = scaled_mass(t.W, p32);
+                t.amount = need < 1 ? 0 : need - 1;
+            } else {
+                t.W = min(t.W, t.least);
+                t.amount = scaled_mass(t.W, u);
+            }
+            if (t.head) {
+                found = find_in_list(s.list, 0, t.head_count, 0, 0, t.by_count, t.amount);
+                have = true;
+                continue;
+            }
+            const Bucket b = find_bucket(s.coarse, t.by_count, t.amount);
+            t.bucket = b.at;
+            t.mass = b.mass;
+            t.count = b.count;
+            t.lo = key_below(b.at);
+            t.hi = key_above(b.at);
+            t.planned = t.goal == kTopP || (t.goal == kTopK && !(p < 1.f));
+            if (!t.planned) {
+                collect(b.at, b.at, 1, 0, t.lo, t.hi);
                 return;
             }
-            have = false;
-            t.pending = kDone;
-            t.W = found.prefix;
-            t.goal = t.goal == kTopK && p < 1.f ? kTopP : kToken;
+            // W will lie in this bucket: but for that the token's bucket is known, and
+            // its tokens are collected in the same pass
+            const Bucket f1 = find_bucket(s.coarse, false, scaled_mass(min(b.mass, t.least), u));
+            const Bucket f2 = find_bucket(s.coarse, false, scaled_mass(min(b.mass + s.coarse.mass(b.at), t.least), u));
+            t.plan_mass = f1.mass;
+            t.plan_b1 = f2.at;
+            if (f2.at < b.at) {
+                collect(b.at, b.at, f1.at, f2.at, 0, t.hi);
+            } else if (f1.at == b.at) {
+                collect(b.at, b.at, 1, 0, t.lo, t.hi);
+            } else {  // the two adjoin: first the one, then the other
+                t.planned = false;
+                collect(b.at, b.at, 1, 0, t.lo, t.hi);
+            }
+            return;
         }
     };
 
-    // ---- passes, the first a histogram up to y = 8 with, where the filters need
-    // it, the sum of the rest ----
-    SampleCommand cmd{kHistogram, 0, kHeadKey, kFirstKey, 0, kFirstShift, 0, 0, whole};
+    // ---- passes, the first the row's histogram ----
+    SampleCommand cmd{kCoarse, 0, NB - 1, 1, 0, 0, kNoMassKey, 0, 0, top_k <= 0 || top_k > kList};
     const T* element = reinterpret_cast<const T*>(held);
     auto y_of = [&](int i) { return __fmul_rn(__fsub_rn(m, to_float(element[i])), inv_t); };
 #pragma unroll 1
@@ -548,85 +587,106 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         // a logit below which no key is below hi: y >= hi once (m - l)/T is above it
         // by more than the roundings
         const float least = m - __uint_as_float(cmd.hi) * temp * 1.00001f - fabsf(m) * 1e-5f;
-        if (cmd.step == kHistogram) {
-            for (int b = tid; b < kBuckets; b += NT) s.low[b] = s.high[b] = s.count[b] = 0u;
-            __syncthreads();
-            uint64_t rest = 0, below = 0;
-            uint32_t tokens = 0;
+        if (cmd.step == kCoarse || cmd.step == kFineStep) {
+            const bool coarse = cmd.step == kCoarse;
+            uint2* parts = coarse ? s.coarse.parts : s.fine.parts;
+            uint32_t* count = coarse ? s.coarse.count : s.fine.count;
+            const int buckets = coarse ? NB : kFine;
+            if (!begin) {
+                for (int b = tid; b < buckets; b += NT) {
+                    parts[b] = make_uint2(0u, 0u);
+                    count[b] = 0u;
+                }
+                sync();  // (a CTA's buckets may be read until here)
+            }
+            const bool counts = top_k > 0, masses = !coarse || cmd.masses;
+            uint64_t below = 0;
 #pragma unroll 1
             for (int c = tid; c < n; c += NT) {
                 const uint4 raw = held[c];
-                if (!cmd.sums && !(chunk_max(raw, T()) >= least)) continue;
+                if (!(chunk_max(raw, T()) >= least)) continue;
                 float x[EPV];
                 Chunk<T>::unpack(raw, x);
 #pragma unroll
                 for (int r = 0; r < EPV; ++r) {
                     const float y = __fmul_rn(__fsub_rn(m, x[r]), inv_t);
-                    const uint32_t key = __float_as_uint(y), w = mass_of(y);
-                    if (key - cmd.lo < cmd.hi - cmd.lo) {
-                        if (w) {
-                            const uint32_t b = key < cmd.lo2 ? 0u : (key - cmd.lo2) >> cmd.shift;
-                            atomicAdd(&s.low[b], w & 0xffffu);
-                            atomicAdd(&s.high[b], w >> 16);
-                            atomicAdd(&s.count[b], 1u);
-                        }
-                    } else if (key >= kHeadKey) {
-                        rest += w;
-                        tokens += w != 0;
+                    if (!(y < kNoMass)) continue;
+                    int b = bucket_of(y);
+                    if (!coarse) {
+                        const uint32_t key = __float_as_uint(y);
+                        if (b != cmd.b0 || key - cmd.lo >= cmd.hi - cmd.lo) continue;
+                        b = int((key - cmd.lo) >> cmd.shift);
                     }
-                    if (y <= limit) below += w;
+                    if (masses) {
+                        const uint32_t w = mass_of(y);
+                        if (w & 0xffffu) atomicAdd(&parts[b].x, w & 0xffffu);
+                        if (w >> 16) atomicAdd(&parts[b].y, w >> 16);
+                        if (y <= limit) below += w;
+                    }
+                    if (counts) atomicAdd(&count[b], 1u);
                 }
             }
-            if (cmd.level == 0) {  // the slice's sums to the first CTA
-                rest = block_reduce<NT>(rest, s.scan, SumOp());
+            if (coarse && mp > 0.f) {  // the slice's mass within the limit, to the first CTA
                 below = block_reduce<NT>(below, s.scan, SumOp());
-                tokens = block_reduce<NT>(tokens, reinterpret_cast<uint32_t*>(s.scan), SumOp());
                 if (tid == 0) {
-                    if (many) {
-                        remote_store(tc::cluster_addr(&s.rest_mass[rank], 0), rest);
-                        remote_store(tc::cluster_addr(&s.min_mass[rank], 0), below);
-                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.rest_tokens[rank], 0)),
-                                     "r"(tokens) : "memory");
-                    } else {
-                        s.rest_mass[0] = rest;
-                        s.min_mass[0] = below;
-                        s.rest_tokens[0] = tokens;
-                    }
+                    if (many) remote_store(tc::cluster_addr(&s.min_mass[rank], 0), below); else s.min_mass[0] = below;
                 }
             }
             sync();
-            // the buckets of all slices, each CTA a share of them, to the first CTA
-            const int share = kBuckets >> log_slices;
+            // the buckets of all slices, each CTA a share of them, to the first CTA, in place
+            const int share = buckets >> log_slices;
 #pragma unroll 1
             for (int b = rank * share + tid; b < (rank + 1) * share; b += NT) {
+                uint64_t w = 0;
+                uint32_t k = 0;
                 if (many) {
-                    uint64_t w = 0;
-                    uint32_t k = 0;
                     for (int r = 0; r < slices; ++r) {
-                        w += (uint64_t(remote_u32(tc::cluster_addr(&s.high[b], r))) << 16) +
-                             remote_u32(tc::cluster_addr(&s.low[b], r));
-                        k += remote_u32(tc::cluster_addr(&s.count[b], r));
+                        const uint64_t x = remote_u64(tc::cluster_addr(parts + b, r));
+                        w += ((x >> 32) << 16) + (x & 0xffffffffu);
+                        if (counts) k += remote_u32(tc::cluster_addr(count + b, r));
                     }
-                    remote_store(tc::cluster_addr(&s.mass[cmd.level][b], 0), w);
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.tokens[cmd.level][b], 0)),
-                                 "r"(k) : "memory");
+                    remote_store(tc::cluster_addr(parts + b, 0), w);
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(count + b, 0)), "r"(k) : "memory");
                 } else {
-                    s.mass[cmd.level][b] = (uint64_t(s.high[b]) << 16) + s.low[b];
-                    s.tokens[cmd.level][b] = s.count[b];
+                    const uint2 x = parts[b];
+                    reinterpret_cast<uint64_t*>(parts)[b] = (uint64_t(x.y) << 16) + x.x;
                 }
             }
         } else if (cmd.step == kCollect) {
             const uint32_t counter = many ? tc::cluster_addr(&s.listed, 0) : 0, list = many ? tc::cluster_addr(s.list, 0) : 0;
+            // all of a warp's finds at once: the place of the first is asked for once
 #pragma unroll 1
-            for (int c = tid; c < n; c += NT) {
-                if (!(chunk_max(held[c], T()) >= least)) continue;
-#pragma unroll 1
-                for (int i = c * EPV; i < (c + 1) * EPV; ++i) {
-                    const uint32_t key = __float_as_uint(y_of(i));
-                    if (key - cmd.lo >= cmd.hi - cmd.lo && key - cmd.lo2 >= cmd.hi2 - cmd.lo2) continue;
-                    const uint64_t entry = (uint64_t(key) << 32) | uint32_t(base + i);
-                    const uint32_t at = many ? remote_add(counter, 1u) : atomicAdd(&s.listed, 1u);
-                    if (at >= kList) continue;
+            for (int c0 = 0; c0 < n; c0 += NT) {
+                const int c = c0 + tid;
+                uint32_t mask = 0;
+                float x[EPV];
+                if (c < n && chunk_max(held[c], T()) >= least) {
+                    Chunk<T>::unpack(held[c], x);
+#pragma unroll
+                    for (int r = 0; r < EPV; ++r) {
+                        const float y = __fmul_rn(__fsub_rn(m, x[r]), inv_t);
+                        const uint32_t key = __float_as_uint(y);
+                        const int b = bucket_of(y);
+                        const bool in = key - cmd.lo < cmd.hi - cmd.lo &&
+                                        ((b >= cmd.b0 && b <= cmd.b1) || (b >= cmd.c0 && b <= cmd.c1));
+                        mask |= uint32_t(in) << r;
+                    }
+                }
+                if (!__any_sync(0xffffffffu, mask != 0)) continue;
+                int at = __popc(mask);
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, at, o);
+                    if (lane >= o) at += y;
+                }
+                const int all = __shfl_sync(0xffffffffu, at, 31);
+                uint32_t start = 0;
+                if (lane == 0) start = many ? remote_add(counter, uint32_t(all)) : atomicAdd(&s.listed, uint32_t(all));
+                at += int(__shfl_sync(0xffffffffu, start, 0)) - __popc(mask);
+                for (; mask; mask &= mask - 1, ++at) {
+                    const int i = c * EPV + __ffs(mask) - 1;
+                    const uint64_t entry = (uint64_t(__float_as_uint(y_of(i))) << 32) | uint32_t(base + i);
+                    if (at >= kList) break;
                     if (many) remote_store(list + at * 8, entry); else s.list[at] = entry;
                 }
             }
@@ -640,8 +700,9 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
             cmd = s.command;
         } else {
             const uint32_t at = tc::cluster_addr(&s.command, 0);
-            cmd = {int(remote_u32(at)), remote_u32(at + 4), remote_u32(at + 8), remote_u32(at + 12), remote_u32(at + 16),
-                   int(remote_u32(at + 20)), remote_u32(at + 24), int(remote_u32(at + 28)), int(remote_u32(at + 32))};
+            cmd = {int(remote_u32(at)), int(remote_u32(at + 4)), int(remote_u32(at + 8)), int(remote_u32(at + 12)),
+                   int(remote_u32(at + 16)), remote_u32(at + 20), remote_u32(at + 24), int(remote_u32(at + 28)),
+                   remote_u32(at + 32), int(remote_u32(at + 36))};
         }
     }
     if (cmd.step == kNth) {  // the nth token with key lo, in index order
@@ -682,7 +743,8 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
 template <class T, int NT>
 void launch_sample(hx_runtime* rt, const SampleArgs& a, uint32_t rows, long chunks, int slices)
 {
-    const size_t smem = ((sizeof(SampleShared) + 15) & ~size_t(15)) + size_t((chunks + slices - 1) / slices) * 16;
+    const size_t smem = ((sizeof(SampleShared<coarse_buckets(NT)>) + 15) & ~size_t(15)) +
+                        size_t((chunks + slices - 1) / slices) * 16;
     require(uint64_t(rows) * slices <= 0x7fffffffu, HX_ERR_UNSUPPORTED, "sampling: too many rows for one call");
     auto kernel = sample_kernel<T, NT>;
     static thread_local int opted[64] = {};
