@@ -76,7 +76,8 @@ __device__ __forceinline__ uint32_t remote_add(uint32_t addr, uint32_t x) {
 constexpr float kNoMass = 24.f;               // tokens beyond have no mass: exp(-24) < 2^-31
 constexpr uint32_t kNoMassKey = 0x41c00000u;  // the bits of 24.0
 constexpr int kFine = 512;                    // buckets of a bucket's own histogram
-constexpr int kList = 128;                    // tokens that are collected and sorted at once
+constexpr int kList = 256;                    // tokens that are collected and sorted at once
+constexpr int kFew = 224;                     // a top_k that is taken from one list
 // Buckets of the row's histogram, equal steps of y: few tokens in each, and few
 // threads of a warp in the same.
 __host__ __device__ constexpr int coarse_buckets(int nt) { return nt == 128 ? 512 : 2048; }
@@ -123,7 +124,7 @@ struct SampleShared {
     float maxima[16];
     uint64_t min_mass[16];  // within min-p's limit
     uint32_t nth_counts[16];
-    uint32_t listed;
+    uint32_t listed, key_min, key_max;  // of what a collection found
     SampleCommand command;
     Thought thought;
 };
@@ -291,7 +292,7 @@ __device__ __noinline__ int list_below(const uint64_t* list, int c, uint32_t key
 // for: the row's histogram, the collection of a bucket's tokens, rarely a bucket's
 // own histogram or the nth of equal tokens.  Bound by the instructions of the passes (about
 // 25 per token in the first, which forms expf of every one) and by the latency
-// between them.  Few-token filters (top_k <= 128) need no masses but those of
+// between them.  Few-token filters (top_k <= kFew) need no masses but those of
 // the tokens they keep: their histogram only counts.
 template <class T, int NT>
 __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8)
@@ -401,7 +402,9 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
     const float limit = mp > 0.f ? fmaxf(-logf(mp), 0.f) : -1.f;
     // the row's bucket of y < kNoMass
     constexpr float kScale = float(NB) / kNoMass;
-    auto bucket_of = [](float y) { return min(int(y * kScale), NB - 1); };
+    auto bucket_of = [](float y) {  // y kScale rounded: the low bits of its sum with 2^23
+        return min(int(__float_as_uint(fmaf(y, kScale, 8388608.f)) - 0x4b000000u), NB - 1);
+    };
     auto key_below = [](int b) { return b <= 1 ? 0u : __float_as_uint(float(b - 1) / kScale); };  // at most those of bucket b
     auto key_above = [](int b) { return min(kNoMassKey, __float_as_uint(float(b + 2) / kScale)); };  // above them
 
@@ -410,7 +413,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         Thought t;
         if (begin) {
             t = Thought{};
-            t.masses = top_k <= 0 || top_k > kList;
+            t.masses = top_k <= 0 || top_k > kFew;
         } else {
             t = s.thought;
         }
@@ -420,6 +423,8 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
             if (lane == 0) {
                 s.command = c;
                 s.listed = 0;
+                s.key_min = 0xffffffffu;
+                s.key_max = 0;
                 s.thought = t;
             }
         };
@@ -429,6 +434,14 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         const uint64_t u = min(fraction32(uniform), uint64_t(0xffffffffu)), p32 = fraction32(p);
         Found found{};
         bool have = false;  // `found` answers the goal
+        auto one_key = [&] {  // the tokens of the only key lo have one mass
+            const uint64_t w = mass_of_key(t.lo), nth = t.by_count ? t.amount - t.count : (t.amount - t.mass) / w;
+            found = {uint64_t(t.lo) << 32, t.mass + (nth + 1) * w};
+            if (t.goal == kToken) {
+                t.amount = nth;
+                t.pending = kNth;
+            }
+        };
         if (t.pending == kCoarse || begin) {  // the row's histogram is there
             lane_prefixes(s.coarse);
             const uint32_t tokens = s.coarse.lane_count[32];
@@ -463,23 +476,26 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                     collect(t.bucket, t.bucket, 1, 0, t.lo, t.hi);
                     return;
                 }
-                // a histogram of this bucket
-                t.shift = 0;
-                while (((t.hi - 1 - t.lo) >> t.shift) >= uint32_t(kFine)) ++t.shift;
-                ask({kFineStep, t.bucket, t.bucket, 1, 0, t.lo, t.hi, t.shift, 0, 0});
-                return;
-            }
-            sort_list(s.list, c);
-            if (t.head) {
-                t.head_count = c;
-                if (mp > 0.f) t.least = list_mass(s.list, c, limit);
-                found = find_in_list(s.list, 0, c, 0, 0, true, t.amount);
+                // a histogram of this bucket's keys, or one key (16-bit logits tie)
+                t.lo = max(t.lo, s.key_min);
+                t.hi = min(t.hi, s.key_max + 1);
+                if (t.hi - t.lo > 1) {
+                    t.shift = 0;
+                    while (((t.hi - 1 - t.lo) >> t.shift) >= uint32_t(kFine)) ++t.shift;
+                    ask({kFineStep, t.bucket, t.bucket, 1, 0, t.lo, t.hi, t.shift, 0, 0});
+                    return;
+                }
+                one_key();
             } else {
-                // the token's tokens first, if they were collected too
-                const int from = t.planned && t.plan_b1 < t.bucket ? list_below(s.list, c, t.lo) : 0;
-                if (t.planned && t.plan_b1 < t.bucket) {
-                    // (lo is a lower bound of the bucket's keys: its neighbour's may reach above)
-                    int f = from;
+                sort_list(s.list, c);
+                if (t.head) {
+                    t.head_count = c;
+                    if (mp > 0.f) t.least = list_mass(s.list, c, limit);
+                    found = find_in_list(s.list, 0, c, 0, 0, true, t.amount);
+                } else if (t.planned && t.plan_b1 < t.bucket) {
+                    // the token's tokens come first in the list (lo is a lower bound of
+                    // the bucket's keys: its neighbour's may reach above)
+                    int f = list_below(s.list, c, t.lo);
                     while (f < c && bucket_of(__uint_as_float(uint32_t(s.list[f] >> 32))) < t.bucket) ++f;
                     found = find_in_list(s.list, f, c, t.mass, t.count, t.by_count, t.amount);
                     t.W = min(found.prefix, t.least);
@@ -487,7 +503,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                     found = find_in_list(s.list, 0, f, t.plan_mass, 0, false, scaled_mass(t.W, u));
                 } else {
                     found = find_in_list(s.list, 0, c, t.mass, t.count, t.by_count, t.amount);
-                    if (t.planned) {  // in one interval
+                    if (t.planned) {  // both in one bucket
                         t.W = min(found.prefix, t.least);
                         t.goal = kToken;
                         found = find_in_list(s.list, 0, c, t.mass, 0, false, scaled_mass(t.W, u));
@@ -506,14 +522,8 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                 collect(t.bucket, t.bucket, 1, 0, t.lo, t.hi);
                 return;
             }
-            // one key: its tokens have one mass
-            const uint64_t w = mass_of_key(t.lo), nth = t.by_count ? t.amount - t.count : (t.amount - t.mass) / w;
-            found = {uint64_t(t.lo) << 32, t.mass + (nth + 1) * w};
+            one_key();
             have = true;
-            if (t.goal == kToken) {
-                t.amount = nth;
-                t.pending = kNth;
-            }
         }
 #pragma unroll 1
         for (;;) {
@@ -579,7 +589,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
     };
 
     // ---- passes, the first the row's histogram ----
-    SampleCommand cmd{kCoarse, 0, NB - 1, 1, 0, 0, kNoMassKey, 0, 0, top_k <= 0 || top_k > kList};
+    SampleCommand cmd{kCoarse, 0, NB - 1, 1, 0, 0, kNoMassKey, 0, 0, top_k <= 0 || top_k > kFew};
     const T* element = reinterpret_cast<const T*>(held);
     auto y_of = [&](int i) { return __fmul_rn(__fsub_rn(m, to_float(element[i])), inv_t); };
 #pragma unroll 1
@@ -654,6 +664,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
             }
         } else if (cmd.step == kCollect) {
             const uint32_t counter = many ? tc::cluster_addr(&s.listed, 0) : 0, list = many ? tc::cluster_addr(s.list, 0) : 0;
+            uint32_t key_min = 0xffffffffu, key_max = 0;
             // all of a warp's finds at once: the place of the first is asked for once
 #pragma unroll 1
             for (int c0 = 0; c0 < n; c0 += NT) {
@@ -670,6 +681,10 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                         const bool in = key - cmd.lo < cmd.hi - cmd.lo &&
                                         ((b >= cmd.b0 && b <= cmd.b1) || (b >= cmd.c0 && b <= cmd.c1));
                         mask |= uint32_t(in) << r;
+                        if (in) {
+                            key_min = min(key_min, key);
+                            key_max = max(key_max, key);
+                        }
                     }
                 }
                 if (!__any_sync(0xffffffffu, mask != 0)) continue;
@@ -688,6 +703,19 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                     const uint64_t entry = (uint64_t(__float_as_uint(y_of(i))) << 32) | uint32_t(base + i);
                     if (at >= kList) break;
                     if (many) remote_store(list + at * 8, entry); else s.list[at] = entry;
+                }
+            }
+            key_min = __reduce_min_sync(0xffffffffu, key_min);
+            key_max = __reduce_max_sync(0xffffffffu, key_max);
+            if (lane == 0 && key_min <= key_max) {
+                if (many) {
+                    asm volatile("red.shared::cluster.min.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.key_min, 0)), "r"(key_min)
+                                 : "memory");
+                    asm volatile("red.shared::cluster.max.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.key_max, 0)), "r"(key_max)
+                                 : "memory");
+                } else {
+                    atomicMin(&s.key_min, key_min);
+                    atomicMax(&s.key_max, key_max);
                 }
             }
         } else {
