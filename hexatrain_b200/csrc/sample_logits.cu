@@ -59,18 +59,23 @@ __device__ __forceinline__ uint32_t remote_u32(uint32_t addr) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
     return x;
 }
-__device__ __forceinline__ uint64_t remote_u64(uint32_t addr) {
-    uint64_t x;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(addr) : "memory");
-    return x;
-}
 __device__ __forceinline__ void remote_store(uint32_t addr, uint64_t x) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(x) : "memory");
+}
+__device__ __forceinline__ void remote_store_u32(uint32_t addr, uint32_t x) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
 }
 __device__ __forceinline__ uint32_t remote_add(uint32_t addr, uint32_t x) {
     uint32_t old;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(x) : "memory");
     return old;
+}
+
+// Adds to a shared word where `if_not` is not 0, without a branch.
+__device__ __forceinline__ void add_shared(uint32_t addr, uint32_t x, uint32_t if_not) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p red.shared::cta.add.u32 [%0], %1;\n\t}" ::"r"(addr),
+                 "r"(x), "r"(if_not)
+                 : "memory");
 }
 
 constexpr float kNoMass = 24.f;               // tokens beyond have no mass: exp(-24) < 2^-31
@@ -105,15 +110,13 @@ struct Thought {
 };
 
 // A histogram: in a slice mass = high 2^16 + low, in the first CTA then the row's
-// masses and counts.
+// masses, high 2^32 + low, and counts.
 template <int N>
 struct Histogram {
-    uint2 parts[N];
-    uint32_t count[N];
+    uint32_t low[N], high[N], count[N];
     uint64_t lane_mass[33];  // before a lane's buckets, and in all
     uint32_t lane_count[33];
-    __device__ __forceinline__ uint64_t& mass(int b) { return reinterpret_cast<uint64_t*>(parts)[b]; }
-    __device__ __forceinline__ uint64_t mass(int b) const { return reinterpret_cast<const uint64_t*>(parts)[b]; }
+    __device__ __forceinline__ uint64_t mass(int b) const { return (uint64_t(high[b]) << 32) | low[b]; }
 };
 template <int NB>
 struct SampleShared {
@@ -176,9 +179,10 @@ __device__ __noinline__ void sort_list(uint64_t* list, int c) {
     for (int k = 2; k <= size; k *= 2)
 #pragma unroll 1
         for (int j = k / 2; j > 0; j /= 2) {
-#pragma unroll 1
-            for (int t = lane; t < size / 2; t += 32) {
-                const int i = 2 * t - (t & (j - 1));
+#pragma unroll
+            for (int q = 0; q < kList / 64; ++q) {
+                const int t = lane + 32 * q, i = 2 * t - (t & (j - 1));
+                if (t >= size / 2) break;
                 const uint64_t a = list[i], b = list[i + j];
                 if ((a > b) == ((i & k) == 0)) {
                     list[i] = b;
@@ -276,17 +280,6 @@ __device__ __noinline__ uint64_t list_mass(const uint64_t* list, int c, float li
     }
     return warp_reduce(w, SumOp());
 }
-// Entries of the sorted list with a key < `key`.
-__device__ __noinline__ int list_below(const uint64_t* list, int c, uint32_t key) {
-    int at = 0;
-#pragma unroll 1
-    for (int j0 = 0; j0 < c; j0 += 32) {
-        const int j = j0 + (threadIdx.x & 31);
-        at += __popc(__ballot_sync(0xffffffffu, j < c && uint32_t(list[j] >> 32) < key));
-    }
-    return at;
-}
-
 // One block per row, or a cluster of them with a slice each, held in shared memory.
 // The first warp of the first CTA thinks, all others make the passes that it asks
 // for: the row's histogram, the collection of a bucket's tokens, rarely a bucket's
@@ -351,8 +344,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         }
     }
     for (int b = tid; b < NB; b += NT) {
-        s.coarse.parts[b] = make_uint2(0u, 0u);
-        s.coarse.count[b] = 0u;
+        s.coarse.low[b] = s.coarse.high[b] = s.coarse.count[b] = 0u;
     }
     bool nan = __syncthreads_or(!(m < INFINITY)) != 0;
     m = block_reduce<NT>(m, reinterpret_cast<float*>(s.scan), MaxOp());
@@ -387,8 +379,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         at = -block_reduce<NT>(-at, reinterpret_cast<int*>(s.scan), MaxOp());
         if (many) {
             if (tid == 0)
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.nth_counts[rank], 0)), "r"(at)
-                             : "memory");
+                remote_store_u32(tc::cluster_addr(&s.nth_counts[rank], 0), at);
             tc::cluster_sync();
             if (rank == 0)
                 for (int r = 0; r < slices; ++r) at = min(at, int(s.nth_counts[r]));
@@ -493,10 +484,14 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                     if (mp > 0.f) t.least = list_mass(s.list, c, limit);
                     found = find_in_list(s.list, 0, c, 0, 0, true, t.amount);
                 } else if (t.planned && t.plan_b1 < t.bucket) {
-                    // the token's tokens come first in the list (lo is a lower bound of
-                    // the bucket's keys: its neighbour's may reach above)
-                    int f = list_below(s.list, c, t.lo);
-                    while (f < c && bucket_of(__uint_as_float(uint32_t(s.list[f] >> 32))) < t.bucket) ++f;
+                    // the token's tokens come first in the list
+                    int f = 0;
+#pragma unroll 1
+                    for (int j0 = 0; j0 < c; j0 += 32) {
+                        const int j = j0 + lane;
+                        f += __popc(__ballot_sync(
+                            0xffffffffu, j < c && bucket_of(__uint_as_float(uint32_t(s.list[j] >> 32))) < t.bucket));
+                    }
                     found = find_in_list(s.list, f, c, t.mass, t.count, t.by_count, t.amount);
                     t.W = min(found.prefix, t.least);
                     t.goal = kToken;
@@ -599,13 +594,14 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         const float least = m - __uint_as_float(cmd.hi) * temp * 1.00001f - fabsf(m) * 1e-5f;
         if (cmd.step == kCoarse || cmd.step == kFineStep) {
             const bool coarse = cmd.step == kCoarse;
-            uint2* parts = coarse ? s.coarse.parts : s.fine.parts;
+            uint32_t* low = coarse ? s.coarse.low : s.fine.low;
+            uint32_t* high = coarse ? s.coarse.high : s.fine.high;
             uint32_t* count = coarse ? s.coarse.count : s.fine.count;
             const int buckets = coarse ? NB : kFine;
+            const uint32_t low_at = tc::smem_u32(low), high_at = tc::smem_u32(high), count_at = tc::smem_u32(count);
             if (!begin) {
                 for (int b = tid; b < buckets; b += NT) {
-                    parts[b] = make_uint2(0u, 0u);
-                    count[b] = 0u;
+                    low[b] = high[b] = count[b] = 0u;
                 }
                 sync();  // (a CTA's buckets may be read until here)
             }
@@ -620,20 +616,20 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
 #pragma unroll
                 for (int r = 0; r < EPV; ++r) {
                     const float y = __fmul_rn(__fsub_rn(m, x[r]), inv_t);
-                    if (!(y < kNoMass)) continue;
                     int b = bucket_of(y);
+                    bool in = y < kNoMass;
                     if (!coarse) {
                         const uint32_t key = __float_as_uint(y);
-                        if (b != cmd.b0 || key - cmd.lo >= cmd.hi - cmd.lo) continue;
-                        b = int((key - cmd.lo) >> cmd.shift);
+                        in = b == cmd.b0 && key - cmd.lo < cmd.hi - cmd.lo;
+                        b = in ? int((key - cmd.lo) >> cmd.shift) : 0;
                     }
                     if (masses) {
-                        const uint32_t w = mass_of(y);
-                        if (w & 0xffffu) atomicAdd(&parts[b].x, w & 0xffffu);
-                        if (w >> 16) atomicAdd(&parts[b].y, w >> 16);
-                        if (y <= limit) below += w;
+                        const uint32_t w = in ? mass_of(y) : 0u;
+                        add_shared(low_at + b * 4, w & 0xffffu, w & 0xffffu);
+                        add_shared(high_at + b * 4, w >> 16, w >> 16);
+                        below += y <= limit ? w : 0u;
                     }
-                    if (counts) atomicAdd(&count[b], 1u);
+                    if (counts) add_shared(count_at + b * 4, 1u, in);
                 }
             }
             if (coarse && mp > 0.f) {  // the slice's mass within the limit, to the first CTA
@@ -651,15 +647,17 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                 uint32_t k = 0;
                 if (many) {
                     for (int r = 0; r < slices; ++r) {
-                        const uint64_t x = remote_u64(tc::cluster_addr(parts + b, r));
-                        w += ((x >> 32) << 16) + (x & 0xffffffffu);
+                        w += (uint64_t(remote_u32(tc::cluster_addr(high + b, r))) << 16) +
+                             remote_u32(tc::cluster_addr(low + b, r));
                         if (counts) k += remote_u32(tc::cluster_addr(count + b, r));
                     }
-                    remote_store(tc::cluster_addr(parts + b, 0), w);
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(count + b, 0)), "r"(k) : "memory");
+                    remote_store_u32(tc::cluster_addr(low + b, 0), uint32_t(w));
+                    remote_store_u32(tc::cluster_addr(high + b, 0), uint32_t(w >> 32));
+                    remote_store_u32(tc::cluster_addr(count + b, 0), k);
                 } else {
-                    const uint2 x = parts[b];
-                    reinterpret_cast<uint64_t*>(parts)[b] = (uint64_t(x.y) << 16) + x.x;
+                    w = (uint64_t(high[b]) << 16) + low[b];
+                    low[b] = uint32_t(w);
+                    high[b] = uint32_t(w >> 32);
                 }
             }
         } else if (cmd.step == kCollect) {
@@ -739,8 +737,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         mine = block_reduce<NT>(mine, reinterpret_cast<uint32_t*>(s.scan), SumOp());
         if (many) {
             if (tid < slices)
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(&s.nth_counts[rank], tid)), "r"(mine)
-                             : "memory");
+                remote_store_u32(tc::cluster_addr(&s.nth_counts[rank], tid), mine);
             tc::cluster_sync();
             for (int r = 0; r < rank; ++r) before += s.nth_counts[r];
         }
