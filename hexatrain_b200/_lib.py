@@ -110,6 +110,11 @@ class SamplingC(C.Structure):
     _fields_ = [("greedy", C.c_uint32), ("temperature", C.c_float), ("top_k", C.c_uint32), ("seed", C.c_uint64)]
 
 
+class DeviceSamplingC(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("seed", C.c_uint64)]
+
+
 class SamplingAuditC(C.Structure):
     _fields_ = [("ok", C.c_uint32), ("logits_finite", C.c_uint32), ("weight_sum", C.c_double),
                 ("probability_sum", C.c_double)]
@@ -210,6 +215,12 @@ SIGNATURES.update({
     "hx_distill_forward_backward_device": (C.c_int, _DISTILL + [C.c_void_p, C.c_float, C.c_void_p, C.c_void_p,
                                                                 C.c_size_t]),
     "hx_sample_logits_device": (C.c_int, _ROWS + [C.c_void_p] * 7),
+    "hx_lm_top_logits_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_float] + [C.c_void_p] * 3),
+    "hx_lm_distill_forward_backward_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_float, C.c_uint32] +
+                                              [C.c_void_p] * 3 + [C.c_float] * 3),
+    "hx_lm_generate_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.POINTER(DeviceSamplingC),
+                                        C.c_void_p, C.c_void_p, C.c_void_p]),
+    "hx_sample_uniform": (C.c_double, [C.c_uint64, C.c_uint64]),
 })
 
 _LIB = None

@@ -13,26 +13,11 @@
 // (tiny_language_model_cpu.cpp:77); that is kd = 0, ce = 1 here.
 #include <cmath>
 
+#include "head_ops.cuh"
 #include "head_stream.cuh"
 
 namespace hx {
 namespace head {
-
-struct DistillArgs {
-    const void* logits;
-    void* d_logits;  // NULL: forward only
-    size_t stride, grad_stride;
-    const float* teacher_values;
-    const int32_t* teacher_indices;
-    const float* teacher_lse;  // NULL: renormalised record
-    const int32_t* labels;     // NULL: no hard targets
-    const float* grad_loss;    // NULL: 1 for every row
-    float* loss;               // NULL in the backward
-    float* stats;              // [rows, 3] logsumexp(l/tau), logsumexp(l), q_T/p_T; may be NULL in the fused form
-    int* err;
-    uint32_t vocab, k;
-    float tau, kd, ce, grad_scale;
-};
 
 // exp and log by the hardware's approximations of 2^x and log2 x: relative
 // (absolute, near 1) errors of about 2^-22, which the rounding of the arguments

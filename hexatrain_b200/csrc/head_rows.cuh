@@ -78,20 +78,16 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, Op op) {
     return r;
 }
 
-// ---- a row held in registers -------------------------------------------------
-// A team of NT threads holds up to 32 NT logits of one row (or of one slice of
-// it: the CTAs of a cluster each hold one), 32 to a thread, so that the row is
-// read from memory once.  The row is seen as 16-byte chunks that are aligned
-// in memory; the first chunk begins `lead` elements before the row, and chunk
-// c holds elements [c EPV - lead, c EPV - lead + EPV).  Thread t holds chunks
-// first + t + j NT, so a warp reads 512 consecutive bytes and the index order
-// is (j, t, element).  Chunks at the ends are read and written by element.
-constexpr int kPerThread = 32;
+// ---- chunks -------------------------------------------------------------------
+// A row is seen as 16-byte chunks that are aligned in memory; the first begins
+// `lead` elements before the row, and chunk c holds elements [c EPV - lead, + EPV).
+// Chunks at the ends are read and written by element.
+constexpr int kPerThread = 32;  // logits of a lane where a warp holds a row in registers
 
 template <class T>
 struct Chunk {
     static constexpr int EPV = 16 / int(sizeof(T));   // elements of a 16-byte chunk
-    static constexpr int N = kPerThread / EPV;         // chunks of a thread
+    static constexpr int N = kPerThread / EPV;        // chunks of kPerThread elements
     static __device__ __forceinline__ void unpack(const uint4& raw, float (&x)[EPV]);
     static __device__ __forceinline__ uint4 pack(const float (&x)[EPV]);
 };
@@ -144,137 +140,6 @@ __device__ __forceinline__ uint4 Chunk<__half>::pack(const float (&x)[8]) {
         w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// Where a team's slice of a row lies.  Whole chunks take the unrolled path; the
-// chunk that begins before the row and the one that ends after it are handled
-// by their one thread, element by element.
-template <class T, int NT>
-struct Slice {
-    static constexpr int EPV = Chunk<T>::EPV, N = Chunk<T>::N;
-    int vocab, lead, first, last, thread;  // chunks [first, last)
-    int mine, w0, w1;                      // this thread's first chunk; whole chunks [w0, w1) of the slice
-    bool aligned;                          // chunks are aligned in memory
-    __device__ __forceinline__ Slice(const T* row, int vocab_, int thread_, int rank, int slices)
-        : vocab(vocab_), lead(int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T))), thread(thread_), aligned(true) {
-        int chunks = (vocab + lead + EPV - 1) / EPV;
-        if (chunks > slices * NT * N) {  // the lead would not fit (kMaxVocab logits, not aligned): by element
-            lead = 0;
-            aligned = false;
-            chunks = (vocab + EPV - 1) / EPV;
-        }
-        const int each = (chunks + slices - 1) / slices;
-        first = min(chunks, rank * each);
-        last = min(chunks, first + each);
-        mine = first + thread;
-        w0 = max(first, lead > 0 ? 1 : 0);
-        w1 = min(last, (vocab + lead) / EPV);
-    }
-    __device__ __forceinline__ int index(int j, int r) const { return (mine + j * NT) * EPV + r - lead; }
-    __device__ __forceinline__ bool holds(int i) const { return i + lead >= first * EPV && i + lead < last * EPV; }
-    __device__ __forceinline__ bool whole(int j) const { return mine + j * NT >= w0 && mine + j * NT < w1; }
-    // The partial chunks of the slice: -1 where there is none.
-    __device__ __forceinline__ int head() const { return first == 0 && w0 == 1 && last > 0 ? 0 : -1; }
-    __device__ __forceinline__ int tail() const {
-        const int c = (vocab + lead) / EPV;
-        return c >= max(first, w0) && c < last && (vocab + lead) % EPV != 0 ? c : -1;
-    }
-
-    // issues the loads of the whole chunks
-    __device__ __forceinline__ void fetch(const T* row, uint4 (&raw)[N]) const {
-        if (!aligned) return;
-        const uint4* p = reinterpret_cast<const uint4*>(row - lead) + mine;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (whole(j)) raw[j] = p[j * NT];
-    }
-    // v[j EPV + r] = element index(j, r), -inf where there is none
-    __device__ __forceinline__ void values(const T* row, const uint4 (&raw)[N], float (&v)[kPerThread]) const {
-        if (!aligned) {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-#pragma unroll
-                for (int r = 0; r < EPV; ++r) {
-                    const int i = index(j, r);
-                    v[j * EPV + r] = mine + j * NT < last && i < vocab ? to_float(row[i]) : -INFINITY;
-                }
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            float x[EPV];
-            Chunk<T>::unpack(raw[j], x);
-            const bool ok = whole(j);
-#pragma unroll
-            for (int r = 0; r < EPV; ++r) v[j * EPV + r] = ok ? x[r] : -INFINITY;
-        }
-        if (const int c = head(); c == 0 && thread == 0)
-            place(row, c, v);
-        if (const int c = tail(); c >= 0 && (c - mine) % NT == 0)
-            place(row, c, v);
-    }
-    __device__ __forceinline__ void place(const T* row, int c, float (&v)[kPerThread]) const {
-        const int at = (c - mine) / NT;
-        float x[EPV];
-#pragma unroll
-        for (int r = 0; r < EPV; ++r) {
-            const int i = c * EPV + r - lead;
-            x[r] = i >= 0 && i < vocab ? to_float(row[i]) : -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-#pragma unroll
-            for (int r = 0; r < EPV; ++r)
-                if (j == at) v[j * EPV + r] = x[r];
-    }
-    // writes v to `out`, by chunks where out is aligned as the row is
-    __device__ __forceinline__ void store(T* out, const float (&v)[kPerThread]) const {
-        if (!aligned || int((reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T)) != lead) {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-#pragma unroll
-                for (int r = 0; r < EPV; ++r) {
-                    const int i = index(j, r);
-                    if (mine + j * NT < last && i >= 0 && i < vocab) out[i] = from_float<T>(v[j * EPV + r]);
-                }
-            return;
-        }
-        uint4* p = reinterpret_cast<uint4*>(out - lead) + mine;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            float x[EPV];
-#pragma unroll
-            for (int r = 0; r < EPV; ++r) x[r] = v[j * EPV + r];
-            if (whole(j)) p[j * NT] = Chunk<T>::pack(x);
-        }
-        if (const int c = head(); c == 0 && thread == 0)
-            write(out, c, v);
-        if (const int c = tail(); c >= 0 && (c - mine) % NT == 0)
-            write(out, c, v);
-    }
-    __device__ __forceinline__ void write(T* out, int c, const float (&v)[kPerThread]) const {
-        const int at = (c - mine) / NT;
-#pragma unroll
-        for (int r = 0; r < EPV; ++r) {
-            float x = 0.f;
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j == at) x = v[j * EPV + r];
-            const int i = c * EPV + r - lead;
-            if (i >= 0 && i < vocab) out[i] = from_float<T>(x);
-        }
-    }
-};
-
-// Split cluster barrier: the first phase shows that every CTA of the cluster
-// has started, so that its shared memory may be written.
-__device__ __forceinline__ void cluster_arrive() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void store_remote(uint32_t addr, float4 x) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w)
-                 : "memory");
 }
 
 // Launch of `rows` teams of `slices` CTAs each, a cluster per row when there
@@ -348,15 +213,6 @@ inline long row_chunks(const void* logits, size_t stride, uint32_t rows, uint32_
     const long lead = same ? long(base % 16) / elem_bytes : epv - 1;
     return (long(vocab) + lead + epv - 1) / epv;
 }
-// Slices of a row of `chunks` chunks: as few as hold it, and more, down to
-// `least` chunks each, while the rows alone would leave SMs idle.
-inline int row_slices(uint32_t rows, long chunks, long held, long least, int sm_count) {
-    int s = 1;
-    while (s < 16 && chunks > held * s) s *= 2;
-    while (s < 8 && long(rows) * s * 2 <= sm_count && chunks / (2 * s) >= least) s *= 2;
-    return s;
-}
-
 inline size_t element_bytes(int dtype)
 {
     require(dtype == HX_DTYPE_F32 || dtype == HX_DTYPE_BF16 || dtype == HX_DTYPE_F16, HX_ERR_ARGUMENT,

@@ -18,6 +18,7 @@
 #include "attention_tc_bwd.cuh"
 #include "attention_tiled.cuh"
 #include "gemm.cuh"
+#include "head_ops.cuh"
 #include "lm_kernels.cuh"
 #include "optim.cuh"
 #include "plans.cuh"
@@ -60,7 +61,7 @@ struct LmPlan {
     size_t w_hi, w_lo, wqkv_hi, wqkv_lo;  // TF32 hi/lo splits of the GEMM weights, refreshed every forward
     size_t tokens, in_tok, tgt_tok, in_ids, tgt_ids, bad;
     std::vector<LayerActs> la;
-    size_t xL, logits, probs, row_loss, row_correct, seq_loss, seq_correct, loss, acc, scalars;
+    size_t xL, logits, probs, row_loss, row_correct, soft_loss, seq_loss, seq_correct, loss, acc, scalars;
     size_t dout, dr, dc, dn, df1, dqkv, ln_part;
     size_t attn_bstat;  // tensor-core attention backward: per (sequence, head, row) sum and D
     size_t diag_lig, diag_hp, diag_dout;
@@ -69,6 +70,7 @@ struct LmPlan {
     int emb_chunks = 1, emb_rows = 1;
     size_t emb_part = 0;
     DeviceBuffer onehot;  // lazily sized staging for the one-hot execute API
+    DeviceBuffer streams; // generation on the device: histories, random numbers, tokens
     hx_optimizer_config opt{};
     int muon_count = 0;
     size_t muon_smem = 0;
@@ -109,7 +111,7 @@ struct LmPlan {
     }
 };
 
-size_t lm_plan_bytes(const LmPlan* p) { return p ? p->arena.block.bytes + p->onehot.bytes : 0; }
+size_t lm_plan_bytes(const LmPlan* p) { return p ? p->arena.block.bytes + p->onehot.bytes + p->streams.bytes : 0; }
 
 bool lm_prepared_config(const hx_runtime* rt, hx_lm_config* cfg, uint32_t* optimizer_kind) {
     if (!rt || !rt->lm) return false;
@@ -358,7 +360,17 @@ void record_bucket(hx_runtime* rt, LmPlan& p, int i, cudaStream_t stream)
         HX_CUDA(cudaEventRecord(p.bucket_ev[size_t(i)], stream));
 }
 
-void forward_backward(hx_runtime* rt, LmPlan& p, const float* W, float* G, float grad_scale, int mode = kFullStep)
+// Soft targets in place of the hard ones (hx_lm_distill_forward_backward_device).
+struct SoftTargets {
+    uint32_t k;
+    const float* values;
+    const int32_t* indices;
+    const float* lse;
+    float temperature, kd_weight, ce_weight;
+};
+
+void forward_backward(hx_runtime* rt, LmPlan& p, const float* W, float* G, float grad_scale, int mode = kFullStep,
+                      const SoftTargets* soft = nullptr)
 {
     const Arena& a = p.arena;
     const int M = p.M, T = p.T, D = p.D, F = p.F, V = p.V, B = p.B;
@@ -449,8 +461,21 @@ void forward_backward(hx_runtime* rt, LmPlan& p, const float* W, float* G, float
     }
     gemm<false, false>(rt, M, V, D, xL, D, W + p.off_out, V, EpiStore{logits, (long)V, 0, 0}, wsplit(p.off_out));
     if (mode == kForwardAllRows) return;
-    ProfScope pce(rt, kTagSoftmaxCe, 4.0 * M * V, 4.0 * 2.0 * M * V);
-    if (V == 1024)
+    if (soft) {
+        // the mean over a sequence's positions is the gradient's 1/T
+        float* row = a.at<float>(p.soft_loss);
+        head::distill(rt, HX_DTYPE_F32, uint32_t(M),
+                      {logits, logits, size_t(V), size_t(V), soft->values, soft->indices, soft->lse, tgt_ids, nullptr, row,
+                       nullptr, nullptr, uint32_t(V), soft->k, soft->temperature, soft->kd_weight, soft->ce_weight,
+                       grad_scale / float(T)},
+                      false);
+        ::hx::pdl_launch(widen_loss_kernel, (M + 255) / 256, 256, 0, s, M, row, a.at<double>(p.row_loss),
+                         a.at<int>(p.row_correct));
+        HX_LAUNCHED(rt);
+    }
+    ProfScope pce(rt, kTagSoftmaxCe, soft ? 0.0 : 4.0 * M * V, soft ? 0.0 : 4.0 * 2.0 * M * V);
+    if (soft) {
+    } else if (V == 1024)
         ::hx::pdl_launch(softmax_ce_vec_kernel<32>, row_grid, 32 * rows_per_block, 0, s, 
             M, T, grad_scale, logits, tgt_ids, p.diag ? a.at<float>(p.probs) : nullptr, logits,
             a.at<double>(p.row_loss), a.at<int>(p.row_correct));
@@ -458,7 +483,7 @@ void forward_backward(hx_runtime* rt, LmPlan& p, const float* W, float* G, float
         ::hx::pdl_launch(softmax_ce_kernel, row_grid, 32 * rows_per_block, 0, s, 
             M, V, T, grad_scale, logits, tgt_ids, p.diag ? a.at<float>(p.probs) : nullptr, logits,
             a.at<double>(p.row_loss), a.at<int>(p.row_correct));
-    HX_LAUNCHED(rt);
+    if (!soft) HX_LAUNCHED(rt);
         pce.end();
     ProfScope plr(rt, kTagReduce, 1.0 * M, 12.0 * M);
     ::hx::pdl_launch(loss_seq_kernel, (B + 7) / 8, 256, 0, s, B, T, a.at<double>(p.row_loss), a.at<int>(p.row_correct),
@@ -651,7 +676,13 @@ void lm_run(hx_runtime* rt, LmPlan& p, const GraphCache::Key& key, F&& body)
     run_cached(rt, p.graphs, key, body);
 }
 
-enum LmGraphKind : uintptr_t { kGraphTrainStep = 1, kGraphForwardBackward = 2, kGraphOptimizer = 3 };
+enum LmGraphKind : uintptr_t {
+    kGraphTrainStep = 1,
+    kGraphForwardBackward = 2,
+    kGraphOptimizer = 3,
+    kGraphDistill = 4,
+    kGraphTopLogits = 5
+};
 
 GraphCache::Key lm_key(LmGraphKind kind, const void* tokens, float grad_scale) {
     GraphCache::Key k{};
@@ -661,6 +692,23 @@ GraphCache::Key lm_key(LmGraphKind kind, const void* tokens, float grad_scale) {
     std::memcpy(&bits, &grad_scale, 4);
     k[2] = bits;
     return k;
+}
+
+// The key with a teacher's record and its scalars.
+GraphCache::Key record_key(LmGraphKind kind, const void* tokens, float grad_scale, const void* values, const void* indices,
+                           const void* lse, uint32_t k, float temperature, float kd_weight, float ce_weight) {
+    GraphCache::Key key = lm_key(kind, tokens, grad_scale);
+    key[3] = reinterpret_cast<uintptr_t>(values);
+    key[4] = reinterpret_cast<uintptr_t>(indices);
+    key[5] = reinterpret_cast<uintptr_t>(lse);
+    key[6] = k;
+    const float x[3] = {temperature, kd_weight, ce_weight};
+    for (int i = 0; i < 3; ++i) {
+        uint32_t bits;
+        std::memcpy(&bits, &x[i], 4);
+        key[7 + i] = bits;
+    }
+    return key;
 }
 
 LmPlan& need_lm(hx_runtime* rt) {
@@ -811,6 +859,7 @@ int hx_lm_prepare(hx_runtime* rt, const hx_lm_config* cfg, uint32_t batch, int d
         p.probs = p.diag ? a.reserve(f * M * V) : 0;
         p.row_loss = a.reserve(sizeof(double) * M);
         p.row_correct = a.reserve(sizeof(int) * M);
+        p.soft_loss = a.reserve(sizeof(float) * M);
         p.seq_loss = a.reserve(sizeof(float) * B);
         p.seq_correct = a.reserve(sizeof(int) * B);
         p.loss = a.reserve(f * 4);
@@ -1089,6 +1138,74 @@ int hx_lm_generate(hx_runtime* rt, const uint32_t* prompts, uint32_t prompt_len,
     });
 }
 
+int hx_lm_generate_device(hx_runtime* rt, const uint32_t* prompts, uint32_t prompt_len, uint32_t max_new,
+                          const hx_device_sampling* sampling, const float* uniform, uint32_t* out, float* log_probs) {
+    return hx_guard(rt, [&] {
+        LmPlan& p = need_lm(rt);
+        require(prompts && sampling && out, HX_ERR_ARGUMENT, "generation: null buffer");
+        require(prompt_len > 0, HX_ERR_ARGUMENT, "PROMPT_EMPTY: prompt is empty");
+        require(p.state_ready, HX_ERR_STATE, "generation before state upload");
+        const uint32_t B = p.B, T = p.T, V = p.V;
+        require(uint64_t(prompt_len) + max_new < (uint64_t(1) << 31) && uint64_t(B) * max_new < (uint64_t(1) << 31),
+                HX_ERR_ARGUMENT, "generation: too many tokens");
+        for (size_t i = 0; i < size_t(B) * prompt_len; ++i)
+            require(prompts[i] < V, HX_ERR_ARGUMENT, "INVALID_TINY_LM_TOKEN: token id >= vocabulary size");
+        if (max_new == 0) return;
+        // random numbers: the caller's, or the host sampler's own (stream b from seed + b)
+        std::vector<float> numbers(size_t(B) * max_new);
+        for (uint32_t step = 0; step < max_new; ++step)
+            for (uint32_t b = 0; b < B; ++b)
+                numbers[size_t(step) * B + b] =
+                    uniform ? uniform[size_t(step) * B + b] : float(hx_sample_uniform(sampling->seed + b, step));
+        const size_t room = size_t(prompt_len) + max_new, n = size_t(B) * max_new;
+        // histories [B, room]; then by step: random numbers, tokens, log-probabilities; the settings [B]
+        const size_t words = B * room + 3 * n + 4 * size_t(B);
+        if (p.streams.bytes < words * 4) p.streams.allocate(words * 4);
+        uint32_t* history = p.streams.as<uint32_t>();
+        float* d_uniform = reinterpret_cast<float*>(history + B * room);
+        int32_t* d_tokens = reinterpret_cast<int32_t*>(d_uniform + n);
+        float* d_log_probs = reinterpret_cast<float*>(d_tokens + n);
+        float* settings = d_log_probs + n;
+        std::vector<float> set(4 * size_t(B));
+        for (uint32_t b = 0; b < B; ++b) {
+            set[b] = sampling->temperature;
+            std::memcpy(&set[B + b], &sampling->top_k, 4);
+            set[2 * size_t(B) + b] = sampling->top_p;
+            set[3 * size_t(B) + b] = sampling->min_p;
+        }
+        const Arena& a = p.arena;
+        const cudaStream_t s = rt->stream;
+        HX_CUDA(cudaMemcpy2DAsync(history, room * 4, prompts, size_t(prompt_len) * 4, size_t(prompt_len) * 4, B,
+                                  cudaMemcpyHostToDevice, s));
+        HX_CUDA(cudaMemcpyAsync(d_uniform, numbers.data(), n * 4, cudaMemcpyHostToDevice, s));
+        HX_CUDA(cudaMemcpyAsync(settings, set.data(), set.size() * 4, cudaMemcpyHostToDevice, s));
+        HX_CUDA(cudaMemsetAsync(a.at<int>(p.bad), 0, sizeof(int), s));
+        for (uint32_t step = 0; step < max_new; ++step) {
+            ::hx::pdl_launch(generation_window_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, s, int(B), int(T), int(room),
+                             int(prompt_len + step), step ? d_tokens + size_t(step - 1) * B : nullptr, history,
+                             a.at<int>(p.in_ids), a.at<int>(p.bad));
+            HX_LAUNCHED(rt);
+            forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), 1.0f, kForwardLastRow);
+            head::sample_logits(rt, HX_DTYPE_F32, B,
+                                {a.at<float>(p.logits), size_t(V), d_uniform + size_t(step) * B, settings,
+                                 reinterpret_cast<int32_t*>(settings + B), settings + 2 * size_t(B), settings + 3 * size_t(B),
+                                 d_tokens + size_t(step) * B, d_log_probs + size_t(step) * B, V});
+        }
+        std::vector<int32_t> tokens(n);
+        std::vector<float> logs(n);
+        HX_CUDA(cudaMemcpyAsync(tokens.data(), d_tokens, n * 4, cudaMemcpyDeviceToHost, s));
+        HX_CUDA(cudaMemcpyAsync(logs.data(), d_log_probs, n * 4, cudaMemcpyDeviceToHost, s));
+        rt->check_device_error();
+        for (uint32_t step = 0; step < max_new; ++step)
+            for (uint32_t b = 0; b < B; ++b) {
+                const int32_t t = tokens[size_t(step) * B + b];
+                if (t < 0) fail(HX_ERR_NONFINITE, "generation step produced non-finite logits on prepared graph");
+                out[size_t(b) * max_new + step] = uint32_t(t);
+                if (log_probs) log_probs[size_t(b) * max_new + step] = logs[size_t(step) * B + b];
+            }
+    });
+}
+
 int hx_lm_state_upload(hx_runtime* rt, const float* params, const float* m, const float* v, const float* buf, size_t pc) {
     return hx_guard(rt, [&] {
         LmPlan& p = need_lm(rt);
@@ -1228,6 +1345,45 @@ int hx_lm_forward_backward_device(hx_runtime* rt, const uint32_t* tokens, float 
                 p.B, p.T, p.V, tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad));
             HX_LAUNCHED(rt);
             forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), grad_scale);
+        });
+    });
+}
+
+int hx_lm_top_logits_device(hx_runtime* rt, const uint32_t* tokens, uint32_t k, float temperature, float* values,
+                            int32_t* indices, float* lse) {
+    return hx_guard(rt, [&] {
+        LmPlan& p = need_lm(rt);
+        require(tokens, HX_ERR_ARGUMENT, "top logits: null tokens");
+        require(p.state_ready, HX_ERR_STATE, "top logits before state upload");
+        const Arena& a = p.arena;
+        lm_run(rt, p, record_key(kGraphTopLogits, tokens, 0.f, values, indices, lse, k, temperature, 0.f, 0.f), [&] {
+            ::hx::pdl_launch(split_tokens_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, rt->stream, p.B, p.T, p.V,
+                             tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad));
+            HX_LAUNCHED(rt);
+            forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), 1.0f, kForwardAllRows);
+            head::top_logits(rt, HX_DTYPE_F32, uint32_t(p.M),
+                             {a.at<float>(p.logits), size_t(p.V), values, indices, lse, nullptr, p.V, k, temperature});
+        });
+    });
+}
+
+int hx_lm_distill_forward_backward_device(hx_runtime* rt, const uint32_t* tokens, float grad_scale, uint32_t k,
+                                          const float* teacher_values, const int32_t* teacher_indices,
+                                          const float* teacher_lse, float temperature, float kd_weight,
+                                          float ce_weight) {
+    return hx_guard(rt, [&] {
+        LmPlan& p = need_lm(rt);
+        require(tokens, HX_ERR_ARGUMENT, "forward_backward: null tokens");
+        require(std::isfinite(grad_scale) && grad_scale > 0.f, HX_ERR_ARGUMENT, "forward_backward: invalid grad_scale");
+        require(p.state_ready, HX_ERR_STATE, "forward_backward before state upload");
+        const Arena& a = p.arena;
+        const SoftTargets soft{k, teacher_values, teacher_indices, teacher_lse, temperature, kd_weight, ce_weight};
+        lm_run(rt, p, record_key(kGraphDistill, tokens, grad_scale, teacher_values, teacher_indices, teacher_lse, k,
+                                 temperature, kd_weight, ce_weight), [&] {
+            ::hx::pdl_launch(split_tokens_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, rt->stream, p.B, p.T, p.V,
+                             tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad));
+            HX_LAUNCHED(rt);
+            forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), grad_scale, kFullStep, &soft);
         });
     });
 }

@@ -24,23 +24,11 @@
 // the bits of y, which order it.
 #include <cmath>
 
+#include "head_ops.cuh"
 #include "head_rows.cuh"
 
 namespace hx {
 namespace head {
-
-struct SampleArgs {
-    const void* logits;
-    size_t stride;
-    const float* uniform;
-    const float* temperature;  // NULL: 1
-    const int32_t* top_k;      // NULL or <= 0: the whole vocabulary
-    const float* top_p;        // NULL or >= 1: off
-    const float* min_p;        // NULL or <= 0: off
-    int32_t* tokens;
-    float* log_probs;  // may be NULL
-    uint32_t vocab;
-};
 
 // floor(mass * f / 2^32) for f <= 2^32
 __device__ __forceinline__ uint64_t scaled_mass(uint64_t mass, uint64_t f) {

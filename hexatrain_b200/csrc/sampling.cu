@@ -37,6 +37,10 @@ uint32_t first_max(const float* logits, uint32_t vocab) {
 
 extern "C" {
 
+double hx_sample_uniform(uint64_t seed, uint64_t step) {
+    return double(mix64(seed + step * 0x9E3779B97F4A7C15ull) >> 11) * 0x1.0p-53;
+}
+
 int hx_sample_next_token(const float* logits, uint32_t vocab, const hx_sampling* s, uint64_t step,
                          uint32_t* token, hx_sampling_audit* audit) {
     if (!logits || !s || !token || vocab == 0 || vocab > 65536) return HX_ERR_ARGUMENT;
@@ -75,7 +79,7 @@ int hx_sample_next_token(const float* logits, uint32_t vocab, const hx_sampling*
         if (audit) *audit = a;
         return HX_ERR_NONFINITE;
     }
-    const double u = double(mix64(s->seed + step * 0x9E3779B97F4A7C15ull) >> 11) * 0x1.0p-53;
+    const double u = hx_sample_uniform(s->seed, step);
     double cumulative = 0.0, psum = 0.0;
     bool selected = false, pfinite = true;
     for (uint32_t i = 0; i < k; ++i) {

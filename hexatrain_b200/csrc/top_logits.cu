@@ -11,21 +11,11 @@
 // host (nicopedia_generation.h:286-395).
 #include <cmath>
 
+#include "head_ops.cuh"
 #include "head_stream.cuh"
 
 namespace hx {
 namespace head {
-
-struct TopArgs {
-    const void* logits;
-    size_t stride;
-    float* values;
-    int32_t* indices;
-    float* lse;  // may be NULL
-    int* err;
-    uint32_t vocab, k;
-    float tau;
-};
 
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, int index) { return (uint64_t(key) << 32) | uint32_t(index); }
 

@@ -753,3 +753,41 @@ class Runtime:
         return self._need() and self._ok(self._lib.hx_sample_logits_device(
             self._rt, dtype, rows, vocab, logits, stride, uniform, temperature, top_k, top_p, min_p, tokens,
             log_probs))
+
+    def lm_top_logits_device(self, tokens_ptr: int, k: int, values: int, indices: int, lse: int = 0,
+                             temperature: float = 1.0) -> bool:
+        """A teacher's record of tokens [batch, T+1]: the forward of the device
+        state and the top logits of every position (hx_lm_top_logits_device)."""
+        return self._need() and self._ok(self._lib.hx_lm_top_logits_device(
+            self._rt, tokens_ptr, k, temperature, values, indices, lse))
+
+    def lm_distill_forward_backward_device(self, tokens_ptr: int, grad_scale: float, k: int, teacher_values: int,
+                                           teacher_indices: int, teacher_lse: int = 0, temperature: float = 1.0,
+                                           kd_weight: float = 1.0, ce_weight: float = 0.0) -> bool:
+        """lm_forward_backward_device with the distillation loss
+        (hx_lm_distill_forward_backward_device)."""
+        return self._need() and self._ok(self._lib.hx_lm_distill_forward_backward_device(
+            self._rt, tokens_ptr, grad_scale, k, teacher_values, teacher_indices, teacher_lse, temperature, kd_weight,
+            ce_weight))
+
+    def lm_generate_device(self, prompts, max_new: int, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                           min_p: float = 0.0, seed: int = 0, uniform=None):
+        """Generation with the tokens sampled on the device: prompts [batch,
+        prompt_len] -> (ids [batch, max_new], log-probabilities), or (None, None)
+        with last_error set.  uniform [max_new, batch]: the random numbers, or
+        None for the host sampler's (hx_lm_generate_device)."""
+        if not self._need():
+            return None, None
+        pr = np.ascontiguousarray(prompts, np.uint32)
+        if pr.ndim == 1:
+            pr = pr[None, :]
+        u = None if uniform is None else _f32(uniform)
+        if pr.shape[0] != self._lm_batch or (u is not None and u.size != max_new * pr.shape[0]):
+            self.last_error = "generation: prompts and random numbers must match the prepared batch"
+            return None, None
+        out = np.zeros((pr.shape[0], max_new), np.uint32)
+        logs = np.zeros((pr.shape[0], max_new), np.float32)
+        s = _lib.DeviceSamplingC(temperature, top_k, top_p, min_p, seed)
+        ok = self._ok(self._lib.hx_lm_generate_device(self._rt, ptr(pr), pr.shape[1], max_new, C.byref(s), ptr(u),
+                                                      ptr(out), ptr(logs)))
+        return (out, logs) if ok else (None, None)

@@ -585,6 +585,38 @@ int hx_sample_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t v
                             size_t stride, const float* uniform, const float* temperature, const int32_t* top_k,
                             const float* top_p, const float* min_p, int32_t* tokens, float* log_probs);
 
+/* -- the same on the prepared LM ------------------------------------------ */
+/* A teacher's record: the forward of the device state on tokens [batch, T+1]
+ * (device, as for hx_lm_forward_backward_device) and the top logits of every
+ * position, values and indices [batch*T*k], lse [batch*T] (may be NULL). */
+int hx_lm_top_logits_device(hx_runtime* rt, const uint32_t* tokens, uint32_t k, float temperature, float* values,
+                            int32_t* indices, float* lse);
+/* hx_lm_forward_backward_device with the distillation loss in place of the
+ * cross-entropy: per sequence the mean over its positions, with the record of a
+ * teacher of the same vocabulary (above) and the tokens that follow as labels.
+ * Gradient buffer, loss slot and bucket events as there; the accuracy reads 0. */
+int hx_lm_distill_forward_backward_device(hx_runtime* rt, const uint32_t* tokens, float grad_scale, uint32_t k,
+                                          const float* teacher_values, const int32_t* teacher_indices,
+                                          const float* teacher_lse, float temperature, float kd_weight,
+                                          float ce_weight);
+/* hx_lm_generate with the tokens sampled on the device: the windows, the
+ * random numbers and the tokens stay there and no step waits for the host.
+ * uniform [max_new*batch] in [0, 1) (host), or NULL for the host sampler's own
+ * numbers, with which greedy and top-k streams draw hx_lm_generate's tokens (but
+ * where a number falls within rounding of a boundary).  log_probs [batch*max_new]
+ * (host, may be NULL): each token's log-probability among the kept ones. */
+typedef struct {
+    float temperature;    /* <= 0 or non-finite: greedy */
+    int32_t top_k;        /* <= 0: the whole vocabulary */
+    float top_p, min_p;   /* >= 1, <= 0: off */
+    uint64_t seed;
+} hx_device_sampling;
+int hx_lm_generate_device(hx_runtime* rt, const uint32_t* prompts, uint32_t prompt_len, uint32_t max_new,
+                          const hx_device_sampling* sampling, const float* uniform, uint32_t* out,
+                          float* log_probs);
+/* The host sampler's random number for a seed and a step (53 bits). */
+double hx_sample_uniform(uint64_t seed, uint64_t step);
+
 #ifdef __cplusplus
 }
 #endif
