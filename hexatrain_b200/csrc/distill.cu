@@ -414,6 +414,7 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
         unsigned exchanges = 0;
         uint32_t phase = 0;
         RingCursor at{0, 0};  // of the row's first slot
+        bool begun = false;
         auto skip = [&](size_t row) {
             if (row < rows)
                 for (int c = span_of(row).chunks(); c > 0; c -= kSlot) at.next(ring);
@@ -449,7 +450,11 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
                     posts[b].o1 = rec.ref * kLog2e;
                 }
                 if (marks) {
-                    // once the row has arrived its named logits leave the sums
+                    // Once the row has arrived its named logits leave the sums.  A slot's
+                    // arrival can be told from the one before it only when that one
+                    // is over: the row before, and with it every earlier one, has arrived.
+                    if (b > 0 || begun) stream_wait(formed + (b > 0 ? b : R) - 1, b > 0 ? phase : phase ^ 1, ws);
+                    begun = true;
                     const int first = at.slot;
                     for (int c = span.chunks(); c > 0; c -= kSlot, at.next(ring)) stream_wait(full + at.slot, at.phase, ws);
                     e.each([&](int, float&, float&, int&, int& pos) {

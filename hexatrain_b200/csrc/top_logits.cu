@@ -212,12 +212,13 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
             if (lane == 0) a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, c, -o));
         }
         float bound;  // at least k logits reach it, and not many more
-        if (k <= 32) {  // the k-th of the 128 maxima of eight logits each
+        // (groups: twice as many as k that have a logit)
+        if (k <= 32 && 16 * k <= V) {  // the k-th of the 128 maxima of eight logits each
             uint32_t key[kPerThread / 8];
 #pragma unroll
             for (int i = 0; i < kPerThread / 8; ++i) key[i] = descending_key(fmaxf(group[2 * i], group[2 * i + 1]));
             bound = from_descending_key(warp_kth(key, k, 4));
-        } else if (k <= 96) {  // of the 256 maxima of four
+        } else if (k <= 96 && 8 * k <= V) {  // of the 256 maxima of four
             uint32_t key[kPerThread / 4];
 #pragma unroll
             for (int i = 0; i < kPerThread / 4; ++i) key[i] = descending_key(group[i]);

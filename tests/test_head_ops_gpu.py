@@ -303,6 +303,77 @@ def test_distill_strides(rt, torch, vocab, pad, shift):
         check_distill(rt, torch, x, dtype, 9, 1.3, 0.7, 0.3, True, some_labels(5, vocab), pad, shift)
 
 
+@pytest.mark.parametrize("rows,vocab,dtype", [(1300, 9001, "f32"), (900, 20011, "f16"), (700, 60013, "f16"),
+                                              (500, 40001, "f32"), (3000, 1500, "f32"), (5000, 700, "bf16")])
+def test_distill_many_rows(rt, torch, rows, vocab, dtype):
+    """Several rows to every block, in a padded buffer: the loss and statistics
+    against 64 bits on the GPU, within the bounds of check_distill."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows)
+    k, tau, kd, ce = 11, 1.5, 0.5, 0.5
+    buf = torch.randn(rows, vocab + 29, device="cuda", generator=gen) * 2
+    view = buf.to({"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype])[:, :vocab]
+    x = view.double()
+    teacher = 0.7 * x.float() + torch.randn(rows, vocab, device="cuda", generator=gen)
+    v, i = torch.topk(teacher, k, dim=1)
+    i32, lse = i.to(torch.int32), torch.logsumexp(teacher / tau, 1)
+    y = torch.randint(0, vocab, (rows,), device="cuda", generator=gen).to(torch.int32)
+    loss, stats = torch.empty(rows, device="cuda"), torch.empty(rows, 3, device="cuda")
+    logp, logq = torch.log_softmax(x / tau, 1), v.double() / tau - lse.double()[:, None]
+    q = logq.exp()
+    rest = logp.exp()
+    rest.scatter_(1, i, 0.0)
+    pt, qt = rest.sum(1), 1.0 - q.sum(1)
+    kl = (q * (logq - logp.gather(1, i))).sum(1) + qt * (qt / pt).log()
+    want = kd * tau ** 2 * kl + ce * (torch.logsumexp(x, 1) - x.gather(1, y.long()[:, None])[:, 0])
+    size = 4 * ULP * (float(x.abs().max()) + 30)
+    slack = (2 * REL + size) * (kd * tau * tau + ce)
+    grad = torch.empty(rows, vocab, device="cuda", dtype=view.dtype)
+    g64 = kd * tau * (logp.exp() * torch.where(rest == 0, 1.0, 1.0 - (qt / pt)[:, None]))
+    g64.scatter_add_(1, i, -kd * tau * q)
+    hard = torch.softmax(x, 1)
+    hard.scatter_add_(1, y.long()[:, None], torch.full((rows, 1), -1.0, device="cuda", dtype=torch.float64))
+    g64 += ce * hard
+    args = (CODES[dtype], rows, vocab, view.data_ptr(), vocab + 29, k, v.data_ptr(), i32.data_ptr(), lse.data_ptr(),
+            y.data_ptr(), tau, kd, ce)
+    for _ in range(3):
+        loss.fill_(-7.0)
+        assert rt.distill_forward_device(*args, loss.data_ptr(), stats.data_ptr()), rt.last_error
+        assert rt.synchronize(), rt.last_error
+        assert bool(((loss.double() - want).abs() <= 4 * slack + 4 * ULP * want.abs()).all())
+        assert bool(((stats[:, 2].double() - qt / pt).abs() <= 1e-4 * (qt / pt).clamp(min=1.0)).all())
+        for fused in (True, False):
+            grad.fill_(9.0)
+            if fused:
+                ok = rt.distill_forward_backward_device(*args, loss.data_ptr(), grad.data_ptr(), vocab)
+            else:
+                ok = rt.distill_backward_device(*args, stats.data_ptr(), grad.data_ptr(), vocab)
+            assert ok and rt.synchronize(), rt.last_error
+            tol = 4 * (2 * REL + size) * (kd * tau + ce) + ROUND[dtype] * g64.abs() + (6e-8 if dtype == "f16" else 0)
+            assert bool(((grad.double() - g64).abs() <= tol).all())
+            assert bool(((loss.double() - want).abs() <= 4 * slack + 4 * ULP * want.abs()).all())
+
+
+@pytest.mark.parametrize("rows,vocab,k,dtype", [(1300, 9001, 30, "f32"), (700, 60013, 100, "f16"), (3000, 1500, 64, "bf16"),
+                                                (9000, 700, 9, "f32"), (5000, 40, 17, "f32"), (400, 130001, 200, "bf16")])
+def test_top_many_rows(rt, torch, rows, vocab, k, dtype):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows)
+    buf = torch.randn(rows, vocab + 3, device="cuda", generator=gen) * 2
+    view = buf.to({"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype])[:, :vocab]
+    order = torch.sort(view.float(), dim=1, descending=True, stable=True)
+    want, lse = order.indices[:, :k].to(torch.int32), torch.logsumexp(view.double(), 1)
+    v, i = torch.empty(rows, k, device="cuda"), torch.empty(rows, k, device="cuda", dtype=torch.int32)
+    s = torch.empty(rows, device="cuda")
+    for _ in range(3):
+        v.fill_(-7.0), i.fill_(-7)
+        assert rt.top_logits_device(CODES[dtype], rows, vocab, view.data_ptr(), vocab + 3, k, v.data_ptr(), i.data_ptr(),
+                                    s.data_ptr()), rt.last_error
+        assert rt.synchronize(), rt.last_error
+        assert torch.equal(i, want) and torch.equal(v, order.values[:, :k])
+        assert bool(((s.double() - lse).abs() <= REL + 4 * ULP * (lse.abs() + 12)).all())
+
+
 @pytest.mark.parametrize("vocab", [50, 1024, 9000])
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_edges(rt, torch, vocab, tail):
