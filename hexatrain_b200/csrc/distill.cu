@@ -19,12 +19,6 @@
 namespace hx {
 namespace head {
 
-// exp and log by the hardware's approximations of 2^x and log2 x: relative
-// (absolute, near 1) errors of about 2^-22, which the rounding of the arguments
-// reaches too.
-__device__ __forceinline__ float exp_fast(float x) { return tc::exp2_approx(x * kLog2e); }
-__device__ __forceinline__ float log_fast(float x) { return __log2f(x) * kLn2; }
-
 // The record's entries, j = lane, lane + 32, ...: index, probability, the
 // student's logit, and the position in the team's slice (-1 where it does not
 // hold the token).  In shared memory, or in the registers of the one warp.
@@ -61,12 +55,12 @@ struct EntriesHeld {
 // The exponentials a call needs: of the soft targets' temperature, of the hard
 // targets, or of both (two), where the temperature makes them differ.
 struct Needs {
-    bool soft, hard, two, tail;
-    float c, inv_tau;  // c: log2(e) times the scale of the first exponential
+    bool soft, hard, two, tail, exact;  // exact: 1 / tau is (tau a power of two)
+    float c, inv_tau;                   // c: log2(e) times the scale of the first exponential
     // `both`: the call writes the statistics of both
     __device__ __forceinline__ Needs(const DistillArgs& a, bool both)
         : soft(both || a.kd != 0.f), hard(both || (a.labels && a.ce != 0.f)), two(soft && hard && a.tau != 1.f),
-          tail(a.teacher_lse != nullptr), inv_tau(1.f / a.tau) {
+          tail(a.teacher_lse != nullptr), exact(a.exact_inverse != 0), inv_tau(1.f / a.tau) {
         c = soft ? kLog2e / a.tau : kLog2e;
     }
 };
@@ -104,8 +98,10 @@ struct Record {
     float l_label, A, B;  // A, B: the scales of the soft and the hard gradient
 };
 
-// One warp forms a row's record: the entries hold the teacher's indices and, as
-// q, its values; `number` the row's numbers; logit(i) reads a logit of the row.
+// One warp forms a row's record, in full precision: 1 - sum q and a KL near 0 keep
+// few of the digits of what they are formed from.  The entries hold the teacher's
+// indices and, as q, its values; `number` the row's numbers; logit(i) reads a logit
+// of the row.
 template <class Span, class Entries, class Logit>
 __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs& n, const Span& span, float number,
                                               Entries& e, Logit logit) {
@@ -118,7 +114,7 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
     rec.l_label = label >= 0 ? logit(label) : 0.f;
     float most = -INFINITY, ref = -INFINITY;
     e.each([&](int, float& t, float& l, int& idx, int& pos) {
-        t *= n.inv_tau;
+        t = n.exact ? t * n.inv_tau : t / a.tau;
         l = 0.f;
         pos = -1;
         if (idx >= V) {
@@ -148,14 +144,14 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
         most = warp_max(most);
         float z = 0.f;
         e.each([&](int, float& t, float&, int& idx, int&) {
-            if (rec.has && idx >= 0) z += exp_fast(t - most);
+            if (rec.has && idx >= 0) z += expf(t - most);
         });
-        log_z = most + log_fast(warp_reduce(z, SumOp()));
+        log_z = most + logf(warp_reduce(z, SumOp()));
     }
     const float o = rec.ref * n.c, o1 = rec.ref * kLog2e;
     e.each([&](int, float& q, float& l, int& idx, int& pos) {
         const float logq = q - log_z;
-        q = rec.has && idx >= 0 ? exp_fast(logq) : 0.f;
+        q = rec.has && idx >= 0 ? expf(logq) : 0.f;
         rec.sq += q;
         if (q > 0.f) rec.kl += q * (logq - (l - rec.ref) * n.inv_tau);
         if (n.tail && pos >= 0) {
@@ -246,14 +242,14 @@ struct RowResult {
     // one lane writes the row's loss and statistics
     __device__ __forceinline__ void write(const DistillArgs& a, const Needs& n, const Record& rec, size_t row, float ref,
                                           float s_out, float s_named, float s_hard, float sq, float kl) const {
-        const float s = s_out + s_named, log_s = log_fast(s) - kLn2 * fmaf(ref, n.c, -o);
+        const float s = s_out + s_named, log_s = logf(s) - kLn2 * fmaf(ref, n.c, -o);
         const float lse_tau = n.soft ? ref * n.inv_tau + log_s : 0.f;
-        const float lse_1 = n.two ? ref + (log_fast(s_hard) - kLn2 * fmaf(ref, kLog2e, -o1)) : n.soft ? lse_tau : ref + log_s;
+        const float lse_1 = n.two ? ref + (logf(s_hard) - kLn2 * fmaf(ref, kLog2e, -o1)) : n.soft ? lse_tau : ref + log_s;
         float loss = 0.f;
         if (a.kd != 0.f && rec.has) {
             // sum q (log q - log p); the entries' share is against rec.ref
             kl += sq * ((ref - rec.ref) * n.inv_tau + log_s);
-            if (ratio > 0.f) kl += fmaxf(1.f - sq, 0.f) * log_fast(ratio);
+            if (ratio > 0.f) kl += fmaxf(1.f - sq, 0.f) * logf(ratio);
             loss = a.kd * a.tau * a.tau * kl;
         }
         if (rec.label >= 0 && a.ce != 0.f) loss += a.ce * (lse_1 - rec.l_label);
@@ -946,6 +942,8 @@ void distill(hx_runtime* rt, int dtype, uint32_t rows, DistillArgs a, bool backw
         require(a.d_logits != a.logits || a.grad_stride == a.stride, HX_ERR_ARGUMENT,
                 "distillation: a gradient in place needs the logits' row stride");
     }
+    int exponent = 0;
+    a.exact_inverse = std::frexp(a.tau, &exponent) == 0.5f;
     a.err = rt->device_error();
     ProfScope prof(rt, kTagSoftmaxCe, 6.0 * rows * a.vocab,
                    double(element_bytes(dtype)) * rows * a.vocab * (a.d_logits ? 2.0 : 1.0));

@@ -34,6 +34,7 @@ struct DistillArgs {
     int* err;
     uint32_t vocab, k;
     float tau, kd, ce, grad_scale;
+    int exact_inverse = 0;  // set by distill(): 1 / tau is exact (tau a power of two)
 };
 // backward: the gradient from a.stats; otherwise the loss, with the gradient where
 // a.d_logits is given.
