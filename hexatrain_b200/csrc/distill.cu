@@ -863,7 +863,8 @@ void launch_stream(hx_runtime* rt, const DistillArgs& a, uint32_t rows, long chu
     auto fits = [&](int s) { return resident * int(((chunks + s - 1) / s + kSlot - 1) / kSlot) + 1 <= ring; };
     int s = 1;
     while (s < 16 && !fits(s)) s *= 2;
-    require(fits(s), HX_ERR_UNSUPPORTED, "distillation: no room for the row");
+    require(resident * int(((chunks + s - 1) / s + kSlot - 1) / kSlot) <= ring && ring >= 1, HX_ERR_UNSUPPORTED,
+            "distillation: no room for the row");  // (the slot more is only for speed)
     // few rows: more slices, down to 8 KB, rather than idle SMs
     while (NT == 512 && s < 8 && long(rows) * s * 2 <= rt->sm_count && chunks / (2 * s) >= 512) s *= 2;
     const StreamShape shape{ring, s, __builtin_ctz(unsigned(s))};
@@ -909,7 +910,7 @@ void launch_distill(hx_runtime* rt, const DistillArgs& a, uint32_t rows)
         else launch_warp<T, 512, 8, kPass>(rt, a, rows);
     } else if (chunks <= 1024) {
         launch_stream<T, 128, kPass>(rt, a, rows, chunks);
-    } else if (chunks <= 2560) {
+    } else if (chunks <= 2048) {
         launch_stream<T, 256, kPass>(rt, a, rows, chunks);
     } else {
         launch_stream<T, 512, kPass>(rt, a, rows, chunks);

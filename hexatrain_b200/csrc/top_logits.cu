@@ -701,7 +701,8 @@ void launch_top_stream(hx_runtime* rt, const TopArgs& a, uint32_t rows, long chu
     while (s < 16 && !fits(s, least)) s *= 2;
     int R = most;
     while (R > 1 && !fits(s, R)) --R;
-    require(fits(s, R), HX_ERR_UNSUPPORTED, "top logits: no room for the row");
+    require(2 * int(((chunks + s - 1) / s + kSlot - 1) / kSlot) <= ring_of(s, R), HX_ERR_UNSUPPORTED,
+            "top logits: no room for the row");  // (the slot more is only for speed)
     while (NT == 512 && s < 8 && long(rows) * s * 2 <= rt->sm_count && chunks / (2 * s) >= 512 && fits(2 * s, R)) s *= 2;
     const TopShape shape{ring_of(s, R), s, __builtin_ctz(unsigned(s)), R};
     const size_t smem = TopMemory<NT, kSlot>(shape.ring, R, int(a.k), s).bytes;
@@ -736,7 +737,7 @@ void launch_top(hx_runtime* rt, const TopArgs& a, uint32_t rows)
         HX_LAUNCHED(rt);
     } else if (chunks <= 1024) {
         launch_top_stream<T, 128>(rt, a, rows, chunks);
-    } else if (chunks <= 2560) {
+    } else if (chunks <= 2048) {
         launch_top_stream<T, 256>(rt, a, rows, chunks);
     } else {
         launch_top_stream<T, 512>(rt, a, rows, chunks);

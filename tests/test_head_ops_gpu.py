@@ -133,6 +133,18 @@ def test_top_ties_and_masks(rt, torch, vocab, kind):
         check_top(rt, torch, x, "bf16", min(vocab, 37))
 
 
+def test_largest_vocabulary_not_aligned(rt, torch):
+    x = normal(7, 2, 262144)
+    check_top(rt, torch, x, "f32", 224, pad=1)
+    check_top(rt, torch, x, "bf16", 256, pad=3, shift=1)
+    view, _ = to_device(torch, x, "f32", 1)
+    out = torch.empty(2, 256, device="cuda")
+    assert not rt.top_logits_device(0, 2, 262144, view.data_ptr(), 262145, 256, out.data_ptr(), out.data_ptr())
+    assert "no room" in rt.last_error
+    check_distill(rt, torch, x, "f32", 256, 1.0, 0.5, 0.5, True, some_labels(2, 262144), 1)
+    check_sample(rt, torch, x, "f32", np.array([0.3, 0.8], np.float32), p=0.9, pad=1)
+
+
 def test_top_not_finite(rt, torch):
     x = normal(3, 4, 2000)
     x[0, 100] = np.inf
