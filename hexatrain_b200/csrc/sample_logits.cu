@@ -273,7 +273,7 @@ __device__ __noinline__ uint64_t list_mass(const uint64_t* list, int c, float li
 // for: the row's histogram, the collection of a bucket's tokens, rarely a bucket's
 // own histogram or the nth of equal tokens.  Bound by the instructions of the passes (about
 // 25 per token in the first, which forms expf of every one) and by the latency
-// between them: 256x32768 float32 57 us, 4096x4096 float16 76 us, one row of 1024
+// between them: 256x32768 float32 57 us, 4096x4096 float16 74 us, one row of 1024
 // 10 us.  Few-token filters (top_k <= kFew) need no masses but those of
 // the tokens they keep: their histogram only counts.
 template <class T, int NT>
@@ -561,7 +561,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
             t.plan_mass = f1.mass;
             t.plan_b1 = f2.at;
             if (f2.at < b.at) {
-                collect(b.at, b.at, f1.at, f2.at, 0, t.hi);
+                collect(b.at, b.at, f1.at, f2.at, key_below(f1.at), t.hi);
             } else if (f1.at == b.at) {
                 collect(b.at, b.at, 1, 0, t.lo, t.hi);
             } else {  // the two adjoin: first the one, then the other
@@ -594,7 +594,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                 }
                 sync();  // (a CTA's buckets may be read until here)
             }
-            const bool counts = top_k > 0, masses = !coarse || cmd.masses;
+            const bool counts = top_k > 0, masses = !coarse || cmd.masses, limited = coarse && mp > 0.f;
             uint64_t below = 0;
 #pragma unroll 1
             for (int c = tid; c < n; c += NT) {
@@ -616,12 +616,12 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                         const uint32_t w = in ? mass_of(y) : 0u;
                         add_shared(low_at + b * 4, w & 0xffffu, w & 0xffffu);
                         add_shared(high_at + b * 4, w >> 16, w >> 16);
-                        below += y <= limit ? w : 0u;
+                        if (limited) below += y <= limit ? w : 0u;
                     }
                     if (counts) add_shared(count_at + b * 4, 1u, in);
                 }
             }
-            if (coarse && mp > 0.f) {  // the slice's mass within the limit, to the first CTA
+            if (limited) {  // the slice's mass within the limit, to the first CTA
                 below = block_reduce<NT>(below, s.scan, SumOp());
                 if (tid == 0) {
                     if (many) remote_store(tc::cluster_addr(&s.min_mass[rank], 0), below); else s.min_mass[0] = below;
@@ -662,15 +662,20 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
                     Chunk<T>::unpack(held[c], x);
 #pragma unroll
                     for (int r = 0; r < EPV; ++r) {
-                        const float y = __fmul_rn(__fsub_rn(m, x[r]), inv_t);
-                        const uint32_t key = __float_as_uint(y);
+                        const uint32_t key = __float_as_uint(__fmul_rn(__fsub_rn(m, x[r]), inv_t));
+                        mask |= uint32_t(key - cmd.lo < cmd.hi - cmd.lo) << r;
+                    }
+                    // of those few, the ones in the buckets
+#pragma unroll 1
+                    for (uint32_t rest = mask; rest; rest &= rest - 1) {
+                        const int r = __ffs(rest) - 1;
+                        const float y = y_of(c * EPV + r);
                         const int b = bucket_of(y);
-                        const bool in = key - cmd.lo < cmd.hi - cmd.lo &&
-                                        ((b >= cmd.b0 && b <= cmd.b1) || (b >= cmd.c0 && b <= cmd.c1));
-                        mask |= uint32_t(in) << r;
-                        if (in) {
-                            key_min = min(key_min, key);
-                            key_max = max(key_max, key);
+                        if ((b >= cmd.b0 && b <= cmd.b1) || (b >= cmd.c0 && b <= cmd.c1)) {
+                            key_min = min(key_min, __float_as_uint(y));
+                            key_max = max(key_max, __float_as_uint(y));
+                        } else {
+                            mask &= ~(1u << r);
                         }
                     }
                 }
