@@ -12,6 +12,7 @@
 #include <cmath>
 
 #include "head_ops.cuh"
+#include "head_plan.cuh"
 #include "head_stream.cuh"
 
 namespace hx {
@@ -303,38 +304,9 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
 // CTA's warp, in turn, merges the CTAs' lists.  Bound
 // by instructions, two looks at every chunk and the row warps' sorts: 2048x131072
 // bfloat16, k 128, 276 us, 1.9 TB/s; 8192x16384 float32, k 64, 146 us, 3.7 TB/s.
-constexpr int kGroups = 512, kTopRing = 64;
-__host__ __device__ constexpr int top_blocks(int nt) { return nt == 128 ? 4 : nt == 256 ? 2 : 1; }
-__host__ __device__ constexpr int top_row_warps(int nt) { return nt == 128 ? 4 : nt == 256 ? 6 : 8; }
-
-// Entries of a row's list (a power of two): the bound lets a quarter more than k pass,
-// nearly twice as many where k is half of the groups.
-__host__ __device__ constexpr int stream_list(int k) { return k <= 64 ? 128 : k <= 128 ? 256 : 512; }
-
-struct TopShape {
-    int ring, slices, log_slices, row_warps;
-};
 struct TopPost {
     float o, bound;
 };
-template <int NT, int kSlot>
-struct TopMemory {
-    size_t bars, part, groups, slots, posts, counts, lists, merge, bytes;
-    __host__ __device__ TopMemory(int ring, int R, int k, int slices) {
-        size_t at = size_t(ring) * kSlot * 16;
-        bars = at; at += size_t(2 * ring + 6 * R) * 8;
-        at = (at + 15) & ~size_t(15);
-        slots = at; at += size_t(R) * 2 * 16 * 16;
-        lists = at; at += size_t(R) * stream_list(k) * 8;
-        merge = at; at += slices > 1 ? size_t(R) * slices * ((k + 1) & ~1) * 8 : 0;
-        groups = at; at += size_t(R) * kGroups * 4;
-        part = at; at += size_t(R) * (NT / 32) * 4;
-        posts = at; at += size_t(R) * 8;
-        counts = at; at += size_t(R) * 4;
-        bytes = (at + 15) & ~size_t(15);
-    }
-};
-
 // The running maxima of a thread's four groups (16-bit types two to a register),
 // and the largest element of one chunk.
 template <class T>
@@ -390,7 +362,7 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_aborted;
     const int k = int(a.k), V = int(a.vocab), ring = shape.ring, slices = shape.slices, R = shape.row_warps;
-    const TopMemory<NT, kSlot> mem(ring, R, k, slices);
+    const TopMemory mem(NT, kSlot, ring, R, k, slices);
     const int room = stream_list(k);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + mem.bars);
     uint64_t* empty = full + ring;
@@ -675,10 +647,11 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
             if (lane == 0) tc::mbar_arrive(collected + gb);
             if (++gb == R) { gb = 0; g_phase ^= 1; }
         };
-        size_t row = team;
-        if (row < rows) add_row(row);
-        for (; row < rows; row += teams) {
-            if (row + teams < rows) add_row(row + teams);
+        const size_t ahead = top_adds_ahead(R) ? teams : 0;
+        size_t next = team;
+        for (size_t row = team; row < rows; row += teams) {
+#pragma unroll 1
+            for (; next <= row + ahead && next < rows; next += teams) add_row(next);
             collect_row(row);
         }
     }
@@ -688,26 +661,13 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
 template <class T, int NT>
 void launch_top_stream(hx_runtime* rt, const TopArgs& a, uint32_t rows, long chunks)
 {
-    constexpr int kPerSm = top_blocks(NT), kSlot = 16 / Chunk<T>::EPV * NT;
+    constexpr int kSlot = 16 / Chunk<T>::EPV * NT;
     const int threads = NT + 32 + 32 * top_row_warps(NT);
-    const size_t limit = 233472 / kPerSm - 1024 - 256;  // shared memory of a block
-    auto ring_of = [&](int s, int R) {
-        const size_t fixed = TopMemory<NT, kSlot>(0, R, int(a.k), s).bytes + 32;
-        return fixed < limit ? int(std::min<size_t>((limit - fixed) / (size_t(kSlot) * 16 + 16), kTopRing)) : 0;
-    };
-    // the ring holds two rows' slices and a slot for the copies ahead; where the
-    // lists of wide records take too much, fewer rows are in flight
-    auto fits = [&](int s, int R) { return 2 * int(((chunks + s - 1) / s + kSlot - 1) / kSlot) + 1 <= ring_of(s, R); };
-    const int most = top_row_warps(NT), least = std::min(most, 3);
-    int s = 1;
-    while (s < 16 && !fits(s, least)) s *= 2;
-    int R = most;
-    while (R > 1 && !fits(s, R)) --R;
-    require(2 * int(((chunks + s - 1) / s + kSlot - 1) / kSlot) <= ring_of(s, R), HX_ERR_UNSUPPORTED,
-            "top logits: no room for the row");  // (the slot more is only for speed)
-    while (NT == 512 && s < 8 && long(rows) * s * 2 <= rt->sm_count && chunks / (2 * s) >= 512 && fits(2 * s, R)) s *= 2;
-    const TopShape shape{ring_of(s, R), s, __builtin_ctz(unsigned(s)), R};
-    const size_t smem = TopMemory<NT, kSlot>(shape.ring, R, int(a.k), s).bytes;
+    const size_t limit = stream_limit(top_blocks(NT));
+    const TopShape shape = top_shape(NT, Chunk<T>::EPV, chunks, int(a.k), long(rows), rt->sm_count);
+    const int s = shape.slices;
+    require(shape.row_warps > 0, HX_ERR_UNSUPPORTED, "top logits: no room for the row");
+    const size_t smem = TopMemory(NT, kSlot, shape.ring, shape.row_warps, int(a.k), s).bytes;
     auto kernel = top_stream_kernel<T, NT>;
     static thread_local int opted[64] = {};
     if (!opted[rt->device & 63]) {
