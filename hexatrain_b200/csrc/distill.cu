@@ -347,7 +347,7 @@ struct StreamMemory {  // offsets into dynamic shared memory
     size_t bars, part, slots, posts, entries, bytes;
     __host__ __device__ StreamMemory(int ring, int k) {
         size_t at = size_t(ring) * kSlot * 16;
-        bars = at; at += size_t(2 * ring + 5 * R) * 8;
+        bars = at; at += size_t(2 * ring + 6 * R) * 8;
         at = (at + 15) & ~size_t(15);
         part = at; at += R * (NT / 32) * 8;
         slots = at; at += R * 2 * 16 * 16;
@@ -395,7 +395,8 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
             tc::mbar_init(summed + i, NW);
             tc::mbar_init(result + i, 1);
             tc::mbar_init(written + i, NW);
-            tc::mbar_init(joined + i, 1);
+            tc::mbar_init(joined + 2 * i, 1);
+            tc::mbar_init(joined + 2 * i + 1, 1);
         }
         tc::fence_mbar_init();
     }
@@ -410,7 +411,6 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
         float4* slots = reinterpret_cast<float4*>(smem + mem.slots) + b * 32;
         const Needs need(a, kPass == kForward);
         const RowNumbers numbers(a, !kSums);
-        unsigned exchanges = 0;
         uint32_t phase = 0;
         RingCursor at{0, 0};  // of the row's first slot
         bool begun = false;
@@ -420,17 +420,8 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
         };
         if (marks)
             for (int i = 0; i < b; ++i) skip(team + i * teams);
-        // what every CTA of the cluster has, to every one of them
-        auto exchange = [&](float4 x) {
-            const int xb = exchanges & 1;
-            if (lane == 0) tc::mbar_arrive_expect_tx(joined + b, 16u * slices);
-            __syncwarp();
-            if (lane < slices)
-                store_async(tc::cluster_addr(slots + xb * 16 + rank, lane), x, tc::cluster_addr(joined + b, lane));
-            stream_wait(joined + b, xb, ws);
-            ++exchanges;
-            return lane < slices ? slots[xb * 16 + lane] : make_float4(0.f, 0.f, 0.f, -INFINITY);
-        };
+        ClusterExchange joins{slots, joined + 2 * b, rank, slices};
+        auto exchange = [&](float4 x) { return joins(x, make_float4(0.f, 0.f, 0.f, -INFINITY), ws); };
         for (size_t row = team + b * teams; row < rows; row += R * teams, phase ^= 1) {
             const Span<T> span = span_of(row);
             const float number = numbers.of(row);

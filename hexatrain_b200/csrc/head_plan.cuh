@@ -14,6 +14,15 @@
 namespace hx {
 namespace head {
 
+// ---- the exchange between the CTAs of a cluster (head_stream.cuh) -------------------
+// Exchange n uses slots and barrier n % 2; it is phase n / 2 of that barrier.  A
+// barrier counts bytes, not senders, and a CTA that is through exchange n sends for
+// n + 1 while another may still wait for bytes of n: on one barrier these would
+// stand in for those.  No CTA sends for n + 2 before every one has sent for n + 1, which
+// it does when it is through n.
+HX_PLAN_FN constexpr int exchange_place(unsigned n) { return int(n & 1); }
+HX_PLAN_FN constexpr unsigned exchange_parity(unsigned n) { return (n >> 1) & 1; }
+
 // ---- top logits of long rows (top_logits.cu) ---------------------------------------
 constexpr int kGroups = 512, kTopRing = 64, kTopSlices = 16;
 // Blocks of nt consumer threads on an SM, and row warps of a block.
@@ -34,7 +43,7 @@ struct TopMemory {
     HX_PLAN_FN constexpr TopMemory(int nt, int slot, int ring, int R, int k, int slices)
         : bars(0), part(0), groups(0), slots(0), posts(0), counts(0), lists(0), merge(0), bytes(0) {
         size_t at = size_t(ring) * slot * 16;
-        bars = at; at += size_t(2 * ring + 6 * R) * 8;
+        bars = at; at += size_t(2 * ring + 7 * R) * 8;
         at = (at + 15) & ~size_t(15);
         slots = at; at += size_t(R) * 2 * 16 * 16;
         lists = at; at += size_t(R) * stream_list(k) * 8;
@@ -64,7 +73,7 @@ inline TopShape top_shape(int nt, int epv, long chunks, int k, long rows, int sm
     const int slot = 16 / epv * nt, most = top_row_warps(nt), least = 3;
     const size_t limit = stream_limit(top_blocks(nt));
     auto ring_of = [&](int s, int R) {
-        const size_t fixed = TopMemory(nt, slot, 0, R, k, s).bytes + 32;
+        const size_t fixed = TopMemory(nt, slot, 0, R, k, s).bytes;
         return fixed < limit ? int(std::min<size_t>((limit - fixed) / (size_t(slot) * 16 + 16), kTopRing)) : 0;
     };
     auto two_rows = [&](int s) { return 2 * int(((chunks + s - 1) / s + slot - 1) / slot); };

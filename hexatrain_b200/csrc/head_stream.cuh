@@ -14,6 +14,7 @@
 // to their end and the block leaves in order.
 #pragma once
 
+#include "head_plan.cuh"
 #include "head_rows.cuh"
 
 namespace hx {
@@ -51,6 +52,25 @@ __device__ __forceinline__ void store_async(uint32_t addr, float4 x, uint32_t ba
         "f"(x.y), "f"(x.z), "f"(x.w), "r"(bar)
         : "memory");
 }
+// A number of each CTA of a cluster, from the same warp of each, to all of them.
+struct ClusterExchange {
+    float4* slots;   // [2][16]
+    uint64_t* bars;  // [2], one arrival each
+    int rank, slices;
+    unsigned n = 0;
+    // lane r gets the number of CTA r, the others `none`
+    __device__ __forceinline__ float4 operator()(float4 x, float4 none, const WaitState& ws) {
+        const int lane = threadIdx.x & 31;
+        uint64_t* bar = bars + exchange_place(n);
+        float4* to = slots + exchange_place(n) * 16;
+        if (lane == 0) tc::mbar_arrive_expect_tx(bar, 16u * slices);
+        __syncwarp();
+        if (lane < slices) store_async(tc::cluster_addr(to + rank, lane), x, tc::cluster_addr(bar, lane));
+        stream_wait(bar, exchange_parity(n), ws);
+        ++n;
+        return lane < slices ? to[lane] : none;
+    }
+};
 // A place in the ring: slots in turn, the phase changes with every round.
 struct RingCursor {
     int slot;

@@ -367,7 +367,7 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + mem.bars);
     uint64_t* empty = full + ring;
     uint64_t *formed = empty + ring, *summed = formed + R, *bounded = summed + R, *collected = bounded + R;
-    uint64_t *joined = collected + R, *merged = joined + R;
+    uint64_t *joined = collected + R, *merged = joined + 2 * R;
     float* part = reinterpret_cast<float*>(smem + mem.part);
     float* groups = reinterpret_cast<float*>(smem + mem.groups);
     TopPost* posts = reinterpret_cast<TopPost*>(smem + mem.posts);
@@ -392,7 +392,8 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
             tc::mbar_init(summed + i, NW);
             tc::mbar_init(bounded + i, 1);
             tc::mbar_init(collected + i, NW);
-            tc::mbar_init(joined + i, 1);
+            tc::mbar_init(joined + 2 * i, 1);
+            tc::mbar_init(joined + 2 * i + 1, 1);
             tc::mbar_init(merged + i, 1);
         }
         tc::fence_mbar_init();
@@ -409,19 +410,10 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
         const int half = (k + 1) & ~1;
         uint64_t* merge = reinterpret_cast<uint64_t*>(smem + mem.merge) + size_t(b) * slices * half;
         const float c = kLog2e / a.tau, inv_tau = 1.f / a.tau;
-        unsigned exchanges = 0;
         uint32_t phase = 0, merges = 0;
         int merger = 0;  // the CTA that merges, in turn
-        auto exchange = [&](float4 x) {
-            const int xb = exchanges & 1;
-            if (lane == 0) tc::mbar_arrive_expect_tx(joined + b, 16u * slices);
-            __syncwarp();
-            if (lane < slices)
-                store_async(tc::cluster_addr(slots + xb * 16 + rank, lane), x, tc::cluster_addr(joined + b, lane));
-            stream_wait(joined + b, xb, ws);
-            ++exchanges;
-            return lane < slices ? slots[xb * 16 + lane] : make_float4(0.f, -INFINITY, -INFINITY, -INFINITY);
-        };
+        ClusterExchange joins{slots, joined + 2 * b, rank, slices};
+        auto exchange = [&](float4 x) { return joins(x, make_float4(0.f, -INFINITY, -INFINITY, -INFINITY), ws); };
         // a logit to take the exponentials against: the largest of 32, loaded a row
         // ahead (a load waits long behind the rows' copies)
         auto sample_of = [&](size_t row) {

@@ -3,6 +3,8 @@
 #include <cstdio>
 #include <cstring>
 #include <map>
+#include <set>
+#include <string>
 #include <tuple>
 #include <vector>
 
@@ -107,8 +109,88 @@ static int top_plans() {
     return bad;
 }
 
+// `kCtas` CTAs of a cluster exchange a number `kTurns` times, in every order in which
+// their steps and the arrivals of what they send can come.  `place` and `parity`: the
+// barrier of exchange n and the phase that is waited for; the slots are n % 2.  True if
+// every CTA reads what was sent for that exchange, and none waits for good.
+constexpr int kCtas = 3, kTurns = 4;
+struct Cluster {
+    signed char turn[kCtas], sent[kCtas];            // exchange, and whether it has sent for it
+    signed char slot[kCtas][2][kCtas];               // exchange whose number lies there
+    signed char phase[kCtas][2], waits[kCtas][2];    // parity; arrivals still wanted
+    signed char bytes[kCtas][2];                     // numbers still wanted
+    unsigned short flying[kCtas];                    // by receiver: bits 3 n % 4 ...: sent by whom
+};
+template <class Place, class Parity>
+static bool exchanges(Place place, Parity parity, size_t* states) {
+    auto key = [](const Cluster& c) { return std::string(reinterpret_cast<const char*>(&c), sizeof(c)); };
+    Cluster first;
+    std::memset(&first, 0, sizeof(first));
+    std::memset(first.slot, -1, sizeof(first.slot));
+    std::memset(first.waits, 1, sizeof(first.waits));
+    std::vector<Cluster> todo{first};
+    std::set<std::string> seen{key(first)};
+    auto settle = [](Cluster& c, int to, int b) {
+        if (c.waits[to][b] == 0 && c.bytes[to][b] == 0) c.phase[to][b] ^= 1, c.waits[to][b] = 1;
+    };
+    while (!todo.empty()) {
+        const Cluster at = todo.back();
+        todo.pop_back();
+        bool moved = false;
+        auto go = [&](const Cluster& c) {
+            moved = true;
+            if (seen.insert(key(c)).second) todo.push_back(c);
+        };
+        for (int i = 0; i < kCtas; ++i) {
+            const int n = at.turn[i];
+            if (n == kTurns) continue;
+            Cluster c = at;
+            if (!at.sent[i]) {  // one arrival, so many bytes wanted; then a number to every CTA
+                const int b = place(n);
+                --c.waits[i][b];
+                c.bytes[i][b] += kCtas;
+                settle(c, i, b);
+                for (int to = 0; to < kCtas; ++to) c.flying[to] |= 1u << (n % 4 * kCtas + i);
+                c.sent[i] = 1;
+                go(c);
+            } else if (at.phase[i][place(n)] != int(parity(n))) {
+                for (int from = 0; from < kCtas; ++from)
+                    if (at.slot[i][n % 2][from] != n) return false;
+                c.turn[i] = n + 1;
+                c.sent[i] = 0;
+                go(c);
+            }
+        }
+        for (int to = 0; to < kCtas; ++to)
+            for (int bit = 0; bit < 4 * kCtas; ++bit)
+                if (at.flying[to] >> bit & 1) {
+                    Cluster c = at;
+                    const int n = bit / kCtas;
+                    c.flying[to] &= ~(1u << bit);
+                    c.slot[to][n % 2][bit % kCtas] = n;
+                    --c.bytes[to][place(n)];
+                    settle(c, to, place(n));
+                    go(c);
+                }
+        if (!moved)
+            for (int i = 0; i < kCtas; ++i)
+                if (at.turn[i] != kTurns) return false;
+    }
+    *states = seen.size();
+    return true;
+}
+static int cluster_exchange() {
+    size_t states = 0;
+    const bool ok = exchanges(exchange_place, exchange_parity, &states);
+    std::printf("%zu states\n", states);
+    // one barrier for all exchanges lets a CTA read a slot before its number is there
+    const bool one = exchanges([](unsigned) { return 0; }, [](unsigned n) { return n & 1; }, &states);
+    return !ok || one;
+}
+
 int main(int argc, char** argv) {
     const char* what = argc > 1 ? argv[1] : "";
     if (!std::strcmp(what, "top")) return top_plans() != 0;
+    if (!std::strcmp(what, "exchange")) return cluster_exchange();
     return 2;
 }

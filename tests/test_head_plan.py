@@ -27,3 +27,9 @@ def test_every_top_logits_call_can_finish(check):
     holds the plan, and consumers, row warps and the ring's producer never wait for one
     another in a circle, however many rows a block takes."""
     check("top")
+
+
+def test_exchange_of_a_cluster_in_every_order(check):
+    """Three CTAs, four exchanges, every order in which sends arrive: each CTA reads
+    what was sent for its exchange (with one barrier for all exchanges it may not)."""
+    check("exchange")
