@@ -429,7 +429,11 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
                 idx = a.teacher_indices[row * k + j];
                 t = a.teacher_values[row * k + j];
             });
-            const Record rec = form_record(a, need, span, number, e, [&](int i) { return to_float(span.row[i]); });
+            // The backward may write over the logits, and nothing tells a CTA how far the others
+            // are: it reads its own slice alone, which is all that its gradient needs.
+            const Record rec = form_record(a, need, span, number, e, [&](int i) {
+                return kSums || span.holds(i) ? to_float(span.row[i]) : 0.f;
+            });
             RowResult res;
             if (!kSums) {
                 res.from_statistics(need, rec, number);

@@ -3,7 +3,7 @@ leave a kernel little room.  Tolerances as in test_head_ops_gpu.py."""
 import numpy as np
 import pytest
 
-from test_head_ops_gpu import CODES, REL, ULP, rt, torch  # noqa: F401
+from test_head_ops_gpu import CODES, REL, ULP, Distill, normal, record_of, rt, some_labels, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,20 @@ def test_top_wide_records_of_many_rows(rt, torch, rows, vocab, k, pad):  # noqa:
         assert rt.synchronize(), rt.last_error
         assert torch.equal(i, want) and torch.equal(v, order.values[:, :k])
         assert bool(((s.double() - lse).abs() <= REL + 4 * ULP * (lse.abs() + 12)).all())
+
+
+# -- the gradient over the logits ------------------------------------------------------
+
+@pytest.mark.parametrize("rows,vocab", [(3, 700), (5, 9001), (6, 40000), (300, 40001), (4, 262144)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_backward_in_place(rt, torch, rows, vocab, tail):  # noqa: F811
+    """The backward over the logits themselves is the one into a buffer of its own, in
+    one block and in a cluster to a row."""
+    x = normal(vocab, rows, vocab, 1.5)
+    for dtype in ("f32", "bf16"):
+        d = Distill(rt, torch, x, dtype, record_of(2, x, 40, 2.0, tail), some_labels(rows, vocab), 2.0, 0.5, 0.5, pad=3)
+        d.forward()
+        want = d.backward(None, 0.5)
+        assert rt.distill_backward_device(*d.args, d.stats.data_ptr(), d.view.data_ptr(), vocab + 3, 0, 0.5), rt.last_error
+        assert rt.synchronize(), rt.last_error
+        assert np.array_equal(d.view.double().cpu().numpy(), want)
