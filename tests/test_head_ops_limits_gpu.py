@@ -3,7 +3,9 @@ leave a kernel little room.  Tolerances as in test_head_ops_gpu.py."""
 import numpy as np
 import pytest
 
-from test_head_ops_gpu import CODES, REL, ULP, Distill, normal, record_of, rt, some_labels, torch  # noqa: F401
+from test_head_ops_gpu import (CODES, REL, ROUND, ULP, Distill, normal, record_of,  # noqa: F401
+                               check_distill, check_top, loss64, lse64, rt,
+                               sample, some_labels, to_device, top, torch)
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +49,54 @@ def test_backward_in_place(rt, torch, rows, vocab, tail):  # noqa: F811
         assert rt.distill_backward_device(*d.args, d.stats.data_ptr(), d.view.data_ptr(), vocab + 3, 0, 0.5), rt.last_error
         assert rt.synchronize(), rt.last_error
         assert np.array_equal(d.view.double().cpu().numpy(), want)
+
+
+# -- a reference far from the row's largest logit ---------------------------------------------
+
+@pytest.mark.parametrize("above", [60.0, 200.0])
+@pytest.mark.parametrize("rows,vocab", [(3, 60), (4, 1000), (4, 1900), (5, 9000), (300, 9001), (5, 40000), (20, 140001)])
+def test_distill_student_far_from_the_teacher(rt, torch, rows, vocab, above):  # noqa: F811
+    """A token that neither record nor label names lies far above all that they do: the
+    sums against a named logit overflow, and are formed again against the maximum."""
+    for tail in (False, True):
+        for tau, kd, ce in ((1.0, 0.6, 0.4), (2.0, 0.5, 0.5), (2.0, 1.0, 0.0)):
+            x = normal(vocab, rows, vocab, 1.0)
+            rec = record_of(6, x, 7, tau, tail)
+            y = some_labels(rows, vocab) if ce else None
+            for r in range(0, rows, 2 if rows < 100 else 7):
+                named = set(rec[1][r].tolist()) | ({int(y[r])} if ce else set())
+                x[r, next(i for i in range(vocab // 2, vocab) if i not in named)] = above * tau
+            check_distill(rt, torch, x, "f32", 7, tau, kd, ce, tail, y, record=rec)
+
+
+@pytest.mark.parametrize("above", [45.0, 200.0])
+@pytest.mark.parametrize("rows,vocab", [(4, 1500), (5, 9000), (300, 9001), (5, 40000), (20, 140001)])
+def test_top_spike_away_from_the_sample(rt, torch, rows, vocab, above):  # noqa: F811
+    x = normal(vocab, rows, vocab, 1.0)
+    x[::2, vocab // 2 + 1] = above
+    for tau in (1.0, 0.5):
+        check_top(rt, torch, x, "f32", 9, tau)
+
+
+# -- sampling: the probabilities of the kept tokens ----------------------------------------------
+
+def test_sample_probabilities_of_the_kept_tokens(rt, torch):  # noqa: F811
+    """Evenly spaced random numbers draw every kept token of more than one step's mass and
+    no other, each with its probability among the kept."""
+    n, vocab = 4096, 50
+    x = np.repeat(normal(8, 1, vocab, 1.0), n, 0)
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    for s in (dict(), dict(k=7), dict(p=0.6), dict(mp=0.2), dict(t=2.0)):
+        tok, lp, l = sample(rt, torch, x, "f32", u, **s)
+        y = (l[0].max() - l[0].astype(np.float64)) / s.get("t", 1.0)
+        order = np.argsort(y, kind="stable")
+        mass = np.exp(-y[order])
+        keep = np.arange(vocab) < s.get("k", vocab)
+        total = mass[keep].sum()
+        keep &= mass.cumsum() - mass < s.get("p", 2.0) * total
+        keep &= mass >= s.get("mp", 0.0)
+        prob = np.zeros(vocab)
+        prob[order[keep]] = mass[keep] / mass[keep].sum()
+        seen = np.bincount(tok, minlength=vocab)
+        assert np.all(prob[seen > 0] > 0) and np.all(prob[seen == 0] <= 1.01 / n)
+        assert np.all(np.abs(lp - np.log(prob[tok])) <= 1e-5)
