@@ -8,7 +8,9 @@
 //         would cancel where the student is sure,
 //   loss = kd tau^2 KL + ce (logsumexp(l) - l_label),
 //   dloss/dl_i = kd tau (p_i c_i - q_i) + ce (softmax(l)_i - [i = label]),
-//   c_i = 1 (renormalised, or i named by the record), 1 - q_T/p_T (elsewhere).
+//   c_i = S (renormalised, or i named by the record), S - q_T/p_T (elsewhere),
+//   S the sum of all the q that the loss has: 1, but sum_j q_j where the bucket is
+//   left out (q_T = 0 or p_T = 0), which may be anything.
 // No counterpart in the reference, whose loss is the hard-label cross-entropy
 // (tiny_language_model_cpu.cpp:77); that is kd = 0, ce = 1 here.
 #include <cmath>
@@ -219,14 +221,19 @@ struct Gradient {
 // inv = 1/s, so that the rounding of o cancels; the logarithm takes its
 // residual, ref c - o, off again.
 struct RowResult {
-    float rest, o, inv, o1, inv1, ratio;
+    float named, rest, o, inv, o1, inv1, ratio;  // named, rest: the soft gradient's factors of p
+    __device__ __forceinline__ void soft_factors(const Needs& n, const Record& rec, float sq) {
+        const float mass = n.tail && ratio == 0.f ? sq : 1.f;
+        named = rec.A * mass;
+        rest = rec.A * (mass - ratio);
+    }
     // statistics written by the forward
-    __device__ __forceinline__ void from_statistics(const Needs& n, const Record& rec, float number) {
+    __device__ __forceinline__ void from_statistics(const Needs& n, const Record& rec, float number, float sq) {
         o = (n.soft ? __shfl_sync(0xffffffffu, number, 3) : __shfl_sync(0xffffffffu, number, 4)) * kLog2e;
         o1 = __shfl_sync(0xffffffffu, number, 4) * kLog2e;
         ratio = __shfl_sync(0xffffffffu, number, 5);
         inv = inv1 = 1.f;
-        rest = rec.A * (1.f - ratio);
+        soft_factors(n, rec, sq);
     }
     __device__ __forceinline__ void from_sums(const Needs& n, const Record& rec, float ref, float s_out, float s_named,
                                               float s_hard, float sq) {
@@ -237,7 +244,7 @@ struct RowResult {
         inv1 = n.two ? __fdividef(1.f, s_hard) : inv;
         ratio = 0.f;
         if (n.tail && n.soft && rec.has && s_out > 0.f) ratio = fmaxf(1.f - sq, 0.f) * __fdividef(s, s_out);
-        rest = rec.A * (1.f - ratio);
+        soft_factors(n, rec, sq);
     }
     // one lane writes the row's loss and statistics
     __device__ __forceinline__ void write(const DistillArgs& a, const Needs& n, const Record& rec, size_t row, float ref,
@@ -266,7 +273,7 @@ struct RowResult {
         return {rec.B * inv1, 0.f, kLog2e, o1, 0.f};
     }
     // the gradient of a token that the record names with probability q
-    // (soft = A) or of an unnamed label (soft = rest, q = 0)
+    // (soft = named) or of an unnamed label (soft = rest, q = 0)
     __device__ __forceinline__ float token(const Needs& n, const Record& rec, float l, float soft, float q, bool is_label) const {
         const float e = tc::exp2_approx(fmaf(l, n.c, -o)) * inv;
         float g = rec.A != 0.f ? soft * e - rec.A * q : 0.f;
@@ -277,7 +284,7 @@ struct RowResult {
     template <class T, class Entries>
     __device__ __forceinline__ void scatter(const Needs& n, const Record& rec, Entries& e, T* d, bool holds_label) const {
         e.each([&](int, float& q, float& l, int& idx, int& pos) {
-            if (pos >= 0) d[idx] = from_float<T>(token(n, rec, l, rec.A, q, idx == rec.label));
+            if (pos >= 0) d[idx] = from_float<T>(token(n, rec, l, named, q, idx == rec.label));
         });
         if ((threadIdx.x & 31) == 0 && holds_label && !rec.label_named)
             d[rec.label] = from_float<T>(token(n, rec, rec.l_label, rest, 0.f, true));
@@ -436,7 +443,7 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
             });
             RowResult res;
             if (!kSums) {
-                res.from_statistics(need, rec, number);
+                res.from_statistics(need, rec, number, warp_reduce(rec.sq, SumOp()));
                 if (lane == 0) posts[b].grad = res.dense(need, rec);
             } else {
                 if (lane == 0) {
@@ -739,7 +746,7 @@ distill_warp_kernel(const DistillArgs a, uint32_t rows)
         __syncwarp();
         const Record rec = form_record(a, need, span, number, e, [&](int i) { return to_float(l[i + span.lead]); });
         RowResult res;
-        if (!kSums) res.from_statistics(need, rec, number);
+        if (!kSums) res.from_statistics(need, rec, number, warp_reduce(rec.sq, SumOp()));
         if (row + teams < rows) {  // the next row's numbers, while this one is worked on
             px = partial_value(span_of(row + teams));
             number = numbers.of(row + teams);

@@ -51,6 +51,100 @@ def test_backward_in_place(rt, torch, rows, vocab, tail):  # noqa: F811
         assert np.array_equal(d.view.double().cpu().numpy(), want)
 
 
+# -- the tail bucket where the student has no mass for it --------------------------------
+
+def soft64(x, record, tau, kd):
+    """(loss, its derivative) of the record's part alone, from the definition: where
+    p_T = 0 or q_T = 0 the bucket is left out, and sum q need not be 1."""
+    tv, ti, tl = record
+    rows = x.shape[0]
+    z = x / tau
+    logp = z - lse64(z)[:, None]
+    p = np.exp(logp)
+    loss, grad = np.zeros(rows), np.zeros_like(x)
+    for r in range(rows):
+        on = ti[r] >= 0
+        ids = ti[r, on]
+        logq = tv[r, on].astype(np.float64) / tau - np.float64(tl[r])
+        q = np.exp(logq)
+        loss[r] = (q * (logq - logp[r, ids]))[q > 0].sum()
+        mass = q.sum()
+        out = np.ones(x.shape[1], bool)
+        out[ids] = False
+        qt, pt = max(0.0, 1.0 - mass), p[r, out].sum()
+        g = np.zeros(x.shape[1])
+        if qt > 0 and pt >= 2.0 ** -126:  # (less is no mass in float32)
+            loss[r] += qt * np.log(qt / pt)
+            g[out] -= qt / pt * p[r, out]
+            mass += qt
+        g += mass * p[r]
+        g[ids] -= q
+        grad[r] = tau * g
+    return kd * tau * tau * loss, kd * grad
+
+
+NO_MASS = ["masked", "below", "sure", "whole"]
+
+
+def no_mass_case(vocab, kind, k=9):
+    """Rows whose tokens outside the record are masked, or too far below to have mass;
+    a record whose entries add up to more than 1; one that names every token."""
+    rows = 5
+    x = normal(vocab + 1, rows, vocab, 1.0)
+    if kind == "whole":
+        k = min(vocab, 256)
+    ti = np.stack([np.random.default_rng(r).permutation(vocab)[:k] for r in range(rows)]).astype(np.int32)
+    tv = normal(k, rows, k, 1.0)
+    tl = (lse64(tv.astype(np.float64) / 2.0) + (-0.3 if kind == "sure" else 0.4)).astype(np.float32)
+    for r in range(rows - 1):  # the last row keeps its tail
+        out = np.ones(vocab, bool)
+        out[ti[r]] = False
+        if kind in ("masked", "whole"):
+            x[r, out] = -np.inf
+        elif kind == "below":
+            x[r, out] -= 2.0 * 120
+    return x, (tv, ti, tl)
+
+
+@pytest.mark.parametrize("kind", NO_MASS)
+@pytest.mark.parametrize("vocab", [60, 1000, 1900, 9000, 40000])
+def test_distill_gradient_without_a_tail(rt, torch, vocab, kind):  # noqa: F811
+    """Loss and gradient, fused and from statistics, with and without labels.  The loss
+    is a sum of q times log-probabilities, each off by REL and the roundings of its size;
+    the gradient one of probabilities, each within 2 REL."""
+    x, rec = no_mass_case(vocab, kind)
+    tau, kd = 2.0, 0.7
+    mass = np.exp(rec[0].astype(np.float64) / tau - rec[2][:, None]).sum(1).max()
+    tol = 4 * (2 * REL + 8 * ULP * 30) * max(1.0, mass)
+    for labels, ce in ((None, 0.0), (np.ascontiguousarray(rec[1][:, 0]), 0.3)):
+        hard = loss64(x.astype(np.float64), rec, labels, tau, 0.0, ce)
+        want, grad = soft64(x.astype(np.float64), rec, tau, kd)
+        want, grad = want + hard[0], grad + hard[2]
+        d = Distill(rt, torch, x, "f32", rec, labels, tau, kd, ce)
+        loss, stats = d.forward()
+        assert np.all(np.abs(loss - want) <= tol * (kd * tau * tau + ce) * 4)
+        assert not stats[:-1, 2].any()
+        for g in (d.backward(), d.fused()[1]):
+            assert np.all(np.abs(g - grad) <= tol * (kd * tau + ce)), np.abs(g - grad).max()
+            assert np.all(np.abs(g.sum(1)) <= tol * (kd * tau + ce) * 4)  # a softmax's gradient
+
+
+@pytest.mark.parametrize("kind", ["masked", "sure"])
+def test_distill_gradient_without_a_tail_against_differences(rt, torch, kind):  # noqa: F811
+    """Central differences of the 64-bit loss, as for the rows with a tail."""
+    x, rec = no_mass_case(40, kind)
+    tau, kd, h = 2.0, 0.7, 1e-4
+    d = Distill(rt, torch, x, "f32", rec, None, tau, kd, 0.0)
+    _, g = d.fused()
+    num = np.zeros_like(g)
+    for i in range(40):
+        up, down = d.x64.copy(), d.x64.copy()
+        up[:, i] += h
+        down[:, i] -= h
+        num[:, i] = (loss64(up, rec, None, tau, kd, 0.0)[0] - loss64(down, rec, None, tau, kd, 0.0)[0]) / (2 * h)
+    assert np.all(np.abs(g - num) <= 4 * (2 * REL + 8 * ULP * 40) * 2 + 10 * h * h)
+
+
 # -- a reference far from the row's largest logit ---------------------------------------------
 
 @pytest.mark.parametrize("above", [60.0, 200.0])
