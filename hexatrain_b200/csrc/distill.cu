@@ -268,6 +268,8 @@ struct RowResult {
         }
     }
     __device__ __forceinline__ Gradient dense(const Needs& n, const Record& rec) const {
+        // a row without targets: its sums may be anything (0 inv is NaN for one of -inf)
+        if (rec.A == 0.f && rec.B == 0.f) return {0.f, 0.f, n.c, 0.f, 0.f};
         if (!n.two) return {((n.soft ? rest : 0.f) + (n.hard ? rec.B : 0.f)) * inv, 0.f, n.c, o, 0.f};  // one softmax
         if (rest != 0.f) return {rest * inv, rec.B * inv1, n.c, o, o1};
         return {rec.B * inv1, 0.f, kLog2e, o1, 0.f};

@@ -145,6 +145,32 @@ def test_distill_gradient_without_a_tail_against_differences(rt, torch, kind):  
     assert np.all(np.abs(g - num) <= 4 * (2 * REL + 8 * ULP * 40) * 2 + 10 * h * h)
 
 
+# -- rows without targets ----------------------------------------------------------------
+
+@pytest.mark.parametrize("value", [-np.inf, np.inf, np.nan, np.finfo(np.float32).min])
+@pytest.mark.parametrize("rows,vocab", [(4, 50), (5, 1000), (5, 1900), (7, 9000), (300, 9001), (5, 40000)])
+def test_distill_rows_without_targets_are_zero(rt, torch, rows, vocab, value):  # noqa: F811
+    """Whatever their logits: one odd logit, or all of them."""
+    x = normal(vocab, rows, vocab)
+    x[0, vocab // 3] = value
+    x[1] = value
+    x[2, ::2] = value
+    rec = list(record_of(1, normal(5, rows, vocab), 5, 1.0, True, short=False))
+    y = some_labels(rows, vocab)
+    rec[1][:3] = -1
+    y[:3] = -1
+    for tail in (False, True):
+        for tau, kd, ce, labels in ((1.0, 1.0, 1.0, y), (2.0, 0.5, 0.5, y), (2.0, 1.0, 0.0, None), (1.0, 0.0, 1.0, y)):
+            for dtype in ("f32", "bf16"):
+                d = Distill(rt, torch, x, dtype, (rec[0], rec[1], rec[2] if tail else None), labels, tau, kd, ce)
+                loss, _ = d.forward()
+                back = d.backward()
+                loss2, g = d.fused()
+                for z in (loss[:3], loss2[:3], back[:3], g[:3]):
+                    assert not z.any()
+                assert np.all(np.isfinite(g[3:])) and g[3:].any() and np.all(np.isfinite(loss2[3:]))
+
+
 # -- a reference far from the row's largest logit ---------------------------------------------
 
 @pytest.mark.parametrize("above", [60.0, 200.0])
