@@ -479,9 +479,8 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
                 const float2 p = lane < NW ? part[b * NW + lane] : make_float2(0.f, 0.f);
                 join_sums(make_float4(p.x, rec.soft, p.y + rec.hard, 0.f), s_out, s_named, s_hard);
                 if (slices > 1) join_sums(exchange(make_float4(s_out, s_named, s_hard, 0.f)), s_out, s_named, s_hard);
-                const float all = s_out + s_named + s_hard;
-                if (!(all < 0x1p60f && all > 0.f)) {
-                    // an overflow, or no finite reference: this warp finds the row's
+                if (!sum_serves(s_out + s_named) || (need.two && !sum_serves(s_hard))) {
+                    // an overflow, or no reference of the row's: this warp finds the row's
                     // maximum and forms the sums against it
                     const int e0 = max(0, span.first * EPV - span.lead), e1 = min(V, span.last * EPV - span.lead);
                     float m = -INFINITY;
@@ -781,9 +780,8 @@ distill_warp_kernel(const DistillArgs a, uint32_t rows)
 #pragma unroll 1
                 for (p += lane; p < chunks; p += 32) add(from[p - lane]);
                 join_sums(make_float4(x.soft, soft, x.hard + hard, 0.f), s_out, s_named, s_hard);
-                const float all = s_out + s_named + s_hard;
-                if (again || (all < 0x1p60f && all > 0.f)) break;
-                // an overflow, or no finite reference: against the row's maximum
+                if (again || (sum_serves(s_out + s_named) && (!need.two || sum_serves(s_hard)))) break;
+                // an overflow, or no reference of the row's: against the row's maximum
                 float m = -INFINITY;
                 for (int i = lane; i < chunks * EPV; i += 32) m = fmaxf(m, to_float(l[i]));
                 e.each([&](int, float&, float& x, int&, int& pos) {

@@ -43,6 +43,12 @@ __device__ __forceinline__ float from_descending_key(uint32_t k) {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
+// Whether a row's sum of exponentials against a reference serves.  Against one of the
+// row's logits it is 1 or more, and too large only where another lies far above.
+// Where the logits looked at are masked the reference is 0 and may lie far above
+// all of the row: below 2^-126 ex2.approx gives 0, so that part of a small sum is missing.
+__device__ __forceinline__ bool sum_serves(float sum) { return sum > 0x1p-60f && sum < 0x1p60f; }
+
 struct SumOp {
     template <class T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
 };

@@ -466,7 +466,7 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 }
                 __syncwarp();
                 if (a.lse) {
-                    if (!(sum < 0x1p60f && sum > 0.f) && top < INFINITY && top > -INFINITY) {
+                    if (!sum_serves(sum) && top < INFINITY && top > -INFINITY) {
                         // the reference was far off: against the maximum
                         ref = top;
                         o = ref * c;

@@ -171,6 +171,41 @@ def test_distill_rows_without_targets_are_zero(rt, torch, rows, vocab, value):  
                 assert np.all(np.isfinite(g[3:])) and g[3:].any() and np.all(np.isfinite(loss2[3:]))
 
 
+# -- log-sum-exp of masked rows ------------------------------------------------------------
+
+def far_masked(rows, vocab, low, rest, value=-np.inf, count=500):
+    """Rows masked but for a few logits about `low`, none at the first token or at any of
+    32 evenly spaced places: two at low, the others at rest."""
+    rng = np.random.default_rng(vocab)
+    places = set((np.arange(32) * vocab // 32).tolist())
+    free = np.array([i for i in range(vocab) if i not in places])
+    x = np.full((rows, vocab), value, np.float32)
+    for r in range(rows):
+        at = rng.permutation(free)[:min(count, len(free) // 2)]
+        x[r, at] = rest
+        x[r, at[:2]] = low
+    return x
+
+
+@pytest.mark.parametrize("value", [-np.inf, np.finfo(np.float32).min])
+@pytest.mark.parametrize("rows,vocab", [(3, 100), (5, 1024), (5, 1030), (700, 2000), (5, 9000), (300, 9001), (4, 40000), (20, 140001)])
+def test_log_sum_exp_of_far_masked_rows(rt, torch, rows, vocab, value):  # noqa: F811
+    for low, rest, tau in ((-87.0, -87.6, 1.0), (-17.4, -17.52, 0.2), (-30.0, -31.0, 1.0), (-120.0, -121.0, 1.0),
+                           (-87.0, -87.6, 2.0)):
+        x = far_masked(rows, vocab, low, rest, value)
+        check_top(rt, torch, x, "f32", 20, tau)
+        tol = REL + 8 * ULP * 130 / min(tau, 1.0)
+        assert np.all(np.abs(top(rt, torch, x, "f32", 20, tau)[2] - lse64(x.astype(np.float64) / tau)) <= tol)
+        # the distillation's statistics, with no logit named but masked ones
+        rec = (np.zeros((rows, 3), np.float32), np.full((rows, 3), -1, np.int32), None)
+        rec[1][::2, 0] = 0
+        d = Distill(rt, torch, x, "f32", rec, np.full(rows, -1, np.int32), tau, 0.5, 0.5)
+        _, stats = d.forward()
+        z = x.astype(np.float64)
+        for got, want in ((stats[:, 0], lse64(z / tau)), (stats[:, 1], lse64(z))):
+            assert np.all(np.abs(got - want) <= tol), np.abs(got - want).max()
+
+
 # -- a reference far from the row's largest logit ---------------------------------------------
 
 @pytest.mark.parametrize("above", [60.0, 200.0])
