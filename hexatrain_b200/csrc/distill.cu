@@ -150,7 +150,7 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
         });
         log_z = most + logf(warp_reduce(z, SumOp()));
     }
-    const float o = rec.ref * n.c, o1 = rec.ref * kLog2e;
+    const float o = offset_against(rec.ref, n.c), o1 = offset_against(rec.ref, kLog2e);
     e.each([&](int, float& q, float& l, int& idx, int& pos) {
         const float logq = q - log_z;
         q = rec.has && idx >= 0 ? expf(logq) : 0.f;
@@ -167,7 +167,7 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
     return rec;
 }
 
-// Sums over a thread's logits: of 2^(l c - o) and of 2^(l log2e - o1).  With a tail
+// Sums over a thread's logits: of 2^(l c - o) and of 2^(l c1 - o1), c1 = log2(e).  With a tail
 // bucket the tokens that the record names have been set to -inf in shared memory
 // before, so that the sum is that of the tail, without cancellation; their own
 // part comes from the record.  The reference logit is one of the row's, so the
@@ -186,29 +186,29 @@ __device__ __forceinline__ float tree_sum(float (&e)[EPV]) {
     return e[0];
 }
 template <int EPV>
-__device__ __forceinline__ void add_chunk(Sums& s, const float (&x)[EPV], const Needs& n, float o, float o1) {
+__device__ __forceinline__ void add_chunk(Sums& s, const float (&x)[EPV], bool two, float c, float o, float c1, float o1) {
     float e[EPV];
 #pragma unroll
-    for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], n.c, -o));
+    for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], c, -o));
     s.soft += tree_sum(e);
-    if (n.two) {
+    if (two) {
 #pragma unroll
-        for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], kLog2e, -o1));
+        for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], c1, -o1));
         s.hard += tree_sum(e);
     }
 }
 
-// A row's gradient: g = A 2^(l c - o) + B 2^(l log2e - o1), the second term only
+// A row's gradient: g = A 2^(l c - o) + B 2^(l c1 - o1), the second term only
 // where both are needed.
 struct Gradient {
-    float A, B, c, o, o1;
+    float A, B, c, o, c1, o1;
     template <int EPV>
     __device__ __forceinline__ void of(const float (&x)[EPV], float (&g)[EPV]) const {
 #pragma unroll
         for (int r = 0; r < EPV; ++r) g[r] = A * tc::exp2_approx(fmaf(x[r], c, -o));
         if (B != 0.f) {
 #pragma unroll
-            for (int r = 0; r < EPV; ++r) g[r] = fmaf(B, tc::exp2_approx(fmaf(x[r], kLog2e, -o1)), g[r]);
+            for (int r = 0; r < EPV; ++r) g[r] = fmaf(B, tc::exp2_approx(fmaf(x[r], c1, -o1)), g[r]);
         } else if (A == 0.f) {  // a row without targets is zero, whatever its logits
 #pragma unroll
             for (int r = 0; r < EPV; ++r) g[r] = 0.f;
@@ -219,18 +219,25 @@ struct Gradient {
 // A row's result, from its sums (forward) or its statistics (backward).  A
 // probability is inv 2^(l c - o): in the forward o = ref c, as in the sums, and
 // inv = 1/s, so that the rounding of o cancels; the logarithm takes its
-// residual, ref c - o, off again.
+// residual, ref c - o, off again.  (c and c1 are the row's: scale_against.)
 struct RowResult {
-    float named, rest, o, inv, o1, inv1, ratio;  // named, rest: the soft gradient's factors of p
+    float named, rest, c, o, inv, c1, o1, inv1, ratio;  // named, rest: the soft gradient's factors of p
     __device__ __forceinline__ void soft_factors(const Needs& n, const Record& rec, float sq) {
         const float mass = n.tail && ratio == 0.f ? sq : 1.f;
         named = rec.A * mass;
         rest = rec.A * (mass - ratio);
     }
+    // A row masked as a whole by a low value: beyond 2^24 its log-sum-exp cannot hold the
+    // logarithm of the number of its logits beside them, and its probabilities count as 0.
+    static __device__ __forceinline__ float offset_of(float lse) {
+        return fabsf(lse) > 0x1p24f && fabsf(lse) < INFINITY ? INFINITY : lse * kLog2e;
+    }
     // statistics written by the forward
     __device__ __forceinline__ void from_statistics(const Needs& n, const Record& rec, float number, float sq) {
-        o = (n.soft ? __shfl_sync(0xffffffffu, number, 3) : __shfl_sync(0xffffffffu, number, 4)) * kLog2e;
-        o1 = __shfl_sync(0xffffffffu, number, 4) * kLog2e;
+        c = n.c;
+        c1 = kLog2e;
+        o = offset_of(n.soft ? __shfl_sync(0xffffffffu, number, 3) : __shfl_sync(0xffffffffu, number, 4));
+        o1 = offset_of(__shfl_sync(0xffffffffu, number, 4));
         ratio = __shfl_sync(0xffffffffu, number, 5);
         inv = inv1 = 1.f;
         soft_factors(n, rec, sq);
@@ -238,8 +245,10 @@ struct RowResult {
     __device__ __forceinline__ void from_sums(const Needs& n, const Record& rec, float ref, float s_out, float s_named,
                                               float s_hard, float sq) {
         const float s = s_out + s_named;
-        o = ref * n.c;
-        o1 = ref * kLog2e;
+        c = scale_against(ref, n.c);
+        c1 = scale_against(ref, kLog2e);
+        o = ref * c;
+        o1 = ref * c1;
         inv = __fdividef(1.f, s);
         inv1 = n.two ? __fdividef(1.f, s_hard) : inv;
         ratio = 0.f;
@@ -249,9 +258,9 @@ struct RowResult {
     // one lane writes the row's loss and statistics
     __device__ __forceinline__ void write(const DistillArgs& a, const Needs& n, const Record& rec, size_t row, float ref,
                                           float s_out, float s_named, float s_hard, float sq, float kl) const {
-        const float s = s_out + s_named, log_s = logf(s) - kLn2 * fmaf(ref, n.c, -o);
-        const float lse_tau = n.soft ? ref * n.inv_tau + log_s : 0.f;
-        const float lse_1 = n.two ? ref + (logf(s_hard) - kLn2 * fmaf(ref, kLog2e, -o1)) : n.soft ? lse_tau : ref + log_s;
+        const float s = s_out + s_named, log_s = logf(s) - kLn2 * fmaf(ref, c, -o);
+        const float log_1 = n.two ? logf(s_hard) - kLn2 * fmaf(ref, c1, -o1) : log_s;
+        const float lse_tau = n.soft ? ref * n.inv_tau + log_s : 0.f, lse_1 = ref + log_1;
         float loss = 0.f;
         if (a.kd != 0.f && rec.has) {
             // sum q (log q - log p); the entries' share is against rec.ref
@@ -259,7 +268,7 @@ struct RowResult {
             if (ratio > 0.f) kl += fmaxf(1.f - sq, 0.f) * logf(ratio);
             loss = a.kd * a.tau * a.tau * kl;
         }
-        if (rec.label >= 0 && a.ce != 0.f) loss += a.ce * (lse_1 - rec.l_label);
+        if (rec.label >= 0 && a.ce != 0.f) loss += a.ce * ((ref - rec.l_label) + log_1);
         if (a.loss) a.loss[row] = loss;
         if (a.stats) {
             a.stats[row * 3] = lse_tau;
@@ -269,17 +278,17 @@ struct RowResult {
     }
     __device__ __forceinline__ Gradient dense(const Needs& n, const Record& rec) const {
         // a row without targets: its sums may be anything (0 inv is NaN for one of -inf)
-        if (rec.A == 0.f && rec.B == 0.f) return {0.f, 0.f, n.c, 0.f, 0.f};
-        if (!n.two) return {((n.soft ? rest : 0.f) + (n.hard ? rec.B : 0.f)) * inv, 0.f, n.c, o, 0.f};  // one softmax
-        if (rest != 0.f) return {rest * inv, rec.B * inv1, n.c, o, o1};
-        return {rec.B * inv1, 0.f, kLog2e, o1, 0.f};
+        if (rec.A == 0.f && rec.B == 0.f) return {0.f, 0.f, c, 0.f, c1, 0.f};
+        if (!n.two) return {((n.soft ? rest : 0.f) + (n.hard ? rec.B : 0.f)) * inv, 0.f, c, o, c1, 0.f};  // one softmax
+        if (rest != 0.f) return {rest * inv, rec.B * inv1, c, o, c1, o1};
+        return {rec.B * inv1, 0.f, c1, o1, c1, 0.f};
     }
     // the gradient of a token that the record names with probability q
     // (soft = named) or of an unnamed label (soft = rest, q = 0)
     __device__ __forceinline__ float token(const Needs& n, const Record& rec, float l, float soft, float q, bool is_label) const {
-        const float e = tc::exp2_approx(fmaf(l, n.c, -o)) * inv;
+        const float e = tc::exp2_approx(fmaf(l, c, -o)) * inv;
         float g = rec.A != 0.f ? soft * e - rec.A * q : 0.f;
-        if (rec.B != 0.f) g += rec.B * ((n.two ? tc::exp2_approx(fmaf(l, kLog2e, -o1)) * inv1 : e) - (is_label ? 1.f : 0.f));
+        if (rec.B != 0.f) g += rec.B * ((n.two ? tc::exp2_approx(fmaf(l, c1, -o1)) * inv1 : e) - (is_label ? 1.f : 0.f));
         return g;
     }
     // One warp writes the record's tokens, and the label, over the dense gradient.
@@ -449,8 +458,8 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
                 if (lane == 0) posts[b].grad = res.dense(need, rec);
             } else {
                 if (lane == 0) {
-                    posts[b].o = rec.ref * need.c;
-                    posts[b].o1 = rec.ref * kLog2e;
+                    posts[b].o = offset_against(rec.ref, need.c);
+                    posts[b].o1 = offset_against(rec.ref, kLog2e);
                 }
                 if (marks) {
                     // Once the row has arrived its named logits leave the sums.  A slot's
@@ -488,11 +497,12 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
                     m = warp_max(m);
                     if (slices > 1) m = warp_max(exchange(make_float4(0.f, 0.f, 0.f, m)).w);
                     ref = m == -INFINITY ? 0.f : m;
+                    const float c = scale_against(ref, need.c), c1 = scale_against(ref, kLog2e), o = ref * c, o1 = ref * c1;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int i = e0 + lane; i < e1; i += 32) {
-                        const float d = to_float(span.row[i]) - ref, y = tc::exp2_approx(d * need.c);
+                        const float l = to_float(span.row[i]), y = tc::exp2_approx(fmaf(l, c, -o));
                         if (marks && e.names(span.position(i))) x.y += y; else x.x += y;
-                        if (need.two) x.z += tc::exp2_approx(d * kLog2e);
+                        if (need.two) x.z += tc::exp2_approx(fmaf(l, c1, -o1));
                     }
                     join_sums(x, s_out, s_named, s_hard);
                     if (slices > 1) join_sums(exchange(make_float4(s_out, s_named, s_hard, 0.f)), s_out, s_named, s_hard);
@@ -530,7 +540,7 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
             auto add = [&](const uint4& raw) {
                 float v[EPV];
                 Chunk<T>::unpack(raw, v);
-                add_chunk<EPV>(x, v, need, o, o1);
+                add_chunk<EPV>(x, v, need.two, need.c, o, kLog2e, o1);
             };
             for (int p0 = 0; p0 < chunks; p0 += kSlot) {
                 stream_wait(full + sums_at.slot, sums_at.phase, ws);
@@ -762,12 +772,14 @@ distill_warp_kernel(const DistillArgs a, uint32_t rows)
                 __syncwarp();
             }
             for (int again = 0;; ++again) {
-                const float o = ref * need.c, o1 = ref * kLog2e;
+                // (the first time with the offsets that the record's part was formed with)
+                const float c = again ? scale_against(ref, need.c) : need.c, c1 = again ? scale_against(ref, kLog2e) : kLog2e;
+                const float o = again ? ref * c : offset_against(ref, c), o1 = again ? ref * c1 : offset_against(ref, c1);
                 Sums x{};
                 auto add = [&](const uint4& raw) {
                     float v[EPV];
                     Chunk<T>::unpack(raw, v);
-                    add_chunk<EPV>(x, v, need, o, o1);
+                    add_chunk<EPV>(x, v, need.two, c, o, c1, o1);
                 };
                 int p = 0;
                 for (; p + 32 * U <= chunks; p += 32 * U) {
@@ -790,12 +802,14 @@ distill_warp_kernel(const DistillArgs a, uint32_t rows)
                 m = warp_max(m);
                 ref = m == -INFINITY ? 0.f : m;
                 soft = hard = 0.f;
-                if (marks)
+                if (marks) {
+                    const float c = scale_against(ref, need.c), c1 = scale_against(ref, kLog2e);
                     e.each([&](int, float&, float& x, int&, int& pos) {
                         if (pos < 0) return;
-                        soft += tc::exp2_approx(fmaf(x, need.c, -ref * need.c));
-                        if (need.two) hard += tc::exp2_approx(fmaf(x, kLog2e, -ref * kLog2e));
+                        soft += tc::exp2_approx(fmaf(x, c, -ref * c));
+                        if (need.two) hard += tc::exp2_approx(fmaf(x, c1, -ref * c1));
                     });
+                }
             }
             const float sq = warp_reduce(rec.sq, SumOp()), kl = warp_reduce(rec.kl, SumOp());
             res.from_sums(need, rec, ref, s_out, s_named, s_hard, sq);

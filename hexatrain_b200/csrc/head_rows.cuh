@@ -49,6 +49,24 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // all of the row: below 2^-126 ex2.approx gives 0, so that part of a small sum is missing.
 __device__ __forceinline__ bool sum_serves(float sum) { return sum > 0x1p-60f && sum < 0x1p60f; }
 
+// Exponentials of a row against one of its logits are 2^(l c - o), c = log2(e) / tau,
+// o = ref c rounded; a row's sum and its uses share o, and its rounding cancels.
+// From kFarOffset on (a row at its type's lowest value) the rounding alone is an
+// exponent of 64 and more.  There two logits are equal or, times c, over 2^7 apart, an
+// exponential is 1 or 0, and a power of two for c gives the same with o exact.
+constexpr float kFarOffset = 0x1p31f;
+__device__ __forceinline__ float scale_against(float ref, float c) {
+    if (fabsf(ref * c) < kFarOffset) return c;
+    const int exponent = int(__float_as_uint(ref) >> 23 & 255u);  // |ref| times the scale in [2^125, 2^126)
+    return __uint_as_float(uint32_t(min(379 - exponent, 254)) << 23);
+}
+// For sums that take c as it is: beyond the bound their exponentials are 0, and no
+// sum serves.
+__device__ __forceinline__ float offset_against(float ref, float c) {
+    const float o = ref * c;
+    return fabsf(o) < kFarOffset ? o : INFINITY;
+}
+
 struct SumOp {
     template <class T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
 };

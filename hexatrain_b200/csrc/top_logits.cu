@@ -205,12 +205,13 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
         }
         top = warp_max(top);
         if (a.lse) {
-            const float ref = fabsf(top) < INFINITY ? top : 0.f, o = ref * c;
+            const float ref = fabsf(top) < INFINITY ? top : 0.f, scale = scale_against(ref, c), o = ref * scale;
             float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < kPerThread; ++i) s[i & 3] += tc::exp2_approx(fmaf(v[i], c, -o));
+            for (int i = 0; i < kPerThread; ++i) s[i & 3] += tc::exp2_approx(fmaf(v[i], scale, -o));
             const float sum = warp_reduce((s[0] + s[1]) + (s[2] + s[3]), SumOp());
-            if (lane == 0) a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, c, -o));
+            if (lane == 0)
+                a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, scale, -o));
         }
         float bound;  // at least k logits reach it, and not many more
         // (groups: twice as many as k that have a logit)
@@ -426,8 +427,8 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                 const int e0 = max(0, span.first * EPV - span.lead), e1 = min(V, span.last * EPV - span.lead);
                 float ref = warp_max(sample);
                 sample = sample_of(row + R * teams);
-                if (!(fabsf(ref) < INFINITY)) ref = 0.f;
-                float o = ref * c;
+                if (!(fabsf(ref * c) < kFarOffset)) ref = 0.f;
+                float scale = c, o = ref * c;
                 if (lane == 0) {
                     posts[b].o = o;
                     counts[b] = 0;
@@ -469,14 +470,16 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                     if (!sum_serves(sum) && top < INFINITY && top > -INFINITY) {
                         // the reference was far off: against the maximum
                         ref = top;
-                        o = ref * c;
+                        scale = scale_against(ref, c);
+                        o = ref * scale;
                         sum = 0.f;
-                        for (int i = e0 + lane; i < e1; i += 32) sum += tc::exp2_approx((to_float(span.row[i]) - ref) * c);
+                        for (int i = e0 + lane; i < e1; i += 32)
+                            sum += tc::exp2_approx(fmaf(to_float(span.row[i]), scale, -o));
                         sum = warp_reduce(sum, SumOp());
                         if (slices > 1) sum = warp_reduce(exchange(make_float4(sum, 0.f, 0.f, 0.f)).x, SumOp());
                     }
                     if (rank == 0 && lane == 0)
-                        a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, c, -o));
+                        a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, scale, -o));
                 }
                 stream_wait(collected + b, phase, ws);
                 int n = counts[b];

@@ -558,7 +558,9 @@ int hx_top_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t voca
  *
  * _forward writes loss[rows] and stats[rows*3] = (logsumexp(l/tau),
  * logsumexp(l), q_T/p_T), which _backward reads; _forward_backward does both in
- * one pass over the logits.  The gradient, in the type of the logits, is
+ * one pass over the logits.  (Beyond 2^24 in size, as for a row masked as a whole by
+ * a low value, a float32 logsumexp does not hold the number of the row's logits:
+ * _backward takes p = 0 there.)  The gradient, in the type of the logits, is
  * grad_scale * grad_loss[row] (1 where grad_loss is NULL) * dloss/dl;
  * d_logits may be the logits themselves (with the same stride). */
 int hx_distill_forward_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,

@@ -206,6 +206,41 @@ def test_log_sum_exp_of_far_masked_rows(rt, torch, rows, vocab, value):  # noqa:
             assert np.all(np.abs(got - want) <= tol), np.abs(got - want).max()
 
 
+# -- rows at the type's lowest value ----------------------------------------------------
+
+LOWEST = [("f32", float(np.finfo(np.float32).min)), ("bf16", -float.fromhex("0x1.fep127")), ("f16", -65504.0),
+          ("f32", -1e30), ("f32", -1e9), ("bf16", -1e9), ("f32", -1e7), ("f32", -1e4), ("f32", 3e38)]
+
+
+@pytest.mark.parametrize("dtype,lowest", LOWEST)
+@pytest.mark.parametrize("vocab", [40, 1000, 1024, 1900, 9000, 40000])
+def test_rows_at_the_lowest_value(rt, torch, vocab, dtype, lowest):  # noqa: F811
+    """Every logit masked by the type's lowest, or another low value: the softmax is uniform.  The same
+    row less its maximum, in 64 bits, has the same loss and gradient."""
+    rows = 5
+    x = np.full((rows, vocab), lowest, np.float32)
+    x[3, 1::2] = -np.inf
+    x[4] = normal(2, 1, vocab)[0]
+    for tau in (1.0, 2.0, 1.5):
+        v, i, s, x64 = top(rt, torch, x, dtype, 7, tau)
+        assert np.array_equal(i[:3], np.broadcast_to(np.arange(7), (3, 7))) and np.array_equal(i[3], np.arange(7) * 2)
+        want = lse64(x64 / tau)
+        assert np.all(np.abs(s - want) <= REL + 8 * ULP * np.abs(want))
+        rec = record_of(3, normal(4, rows, vocab), 6, tau, False, short=False)
+        rec[1][3] = rec[1][3] // 2 * 2
+        rec[1][3, 1:] = -1
+        y = np.array([rec[1][0, 2], 5, -1, 4, 3], np.int32)
+        for kd, ce, labels in ((0.5, 0.5, y), (1.0, 0.0, None), (0.0, 1.0, y)):
+            d = Distill(rt, torch, x, dtype, rec, labels, tau, kd, ce)
+            want, _, grad = loss64(x64 - x64.max(1, keepdims=True), rec, labels, tau, kd, ce)
+            size = (2 * REL + 8 * ULP * 40) * (kd * tau * max(tau, 1.0) + ce)
+            for loss in (d.forward()[0], d.fused()[0]):
+                assert np.all(np.abs(loss - want) <= 4 * size + 4 * ULP * np.abs(want)), (loss, want)
+            g = d.fused()[1]
+            assert np.all(np.abs(g - grad) <= 4 * size + ROUND[dtype] * np.abs(grad) + 6e-8), np.abs(g - grad).max()
+            assert np.all(np.isfinite(d.backward()))
+
+
 # -- a reference far from the row's largest logit ---------------------------------------------
 
 @pytest.mark.parametrize("above", [60.0, 200.0])
