@@ -167,7 +167,7 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
     return rec;
 }
 
-// Sums over a thread's logits: of 2^(l c - o) and of 2^(l c1 - o1), c1 = log2(e).  With a tail
+// Sums over a thread's logits: of 2^(l c - o) and of 2^(l log2e - o1).  With a tail
 // bucket the tokens that the record names have been set to -inf in shared memory
 // before, so that the sum is that of the tail, without cancellation; their own
 // part comes from the record.  The reference logit is one of the row's, so the
@@ -186,14 +186,14 @@ __device__ __forceinline__ float tree_sum(float (&e)[EPV]) {
     return e[0];
 }
 template <int EPV>
-__device__ __forceinline__ void add_chunk(Sums& s, const float (&x)[EPV], bool two, float c, float o, float c1, float o1) {
+__device__ __forceinline__ void add_chunk(Sums& s, const float (&x)[EPV], const Needs& n, float o, float o1) {
     float e[EPV];
 #pragma unroll
-    for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], c, -o));
+    for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], n.c, -o));
     s.soft += tree_sum(e);
-    if (two) {
+    if (n.two) {
 #pragma unroll
-        for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], c1, -o1));
+        for (int r = 0; r < EPV; ++r) e[r] = tc::exp2_approx(fmaf(x[r], kLog2e, -o1));
         s.hard += tree_sum(e);
     }
 }
@@ -245,12 +245,18 @@ struct RowResult {
     __device__ __forceinline__ void from_sums(const Needs& n, const Record& rec, float ref, float s_out, float s_named,
                                               float s_hard, float sq) {
         const float s = s_out + s_named;
-        c = scale_against(ref, n.c);
-        c1 = scale_against(ref, kLog2e);
+        c = n.c;
+        c1 = kLog2e;
+        if (!(fabsf(ref) * fmaxf(n.c, kLog2e) < kFarOffset)) {
+            c = scale_against(ref, n.c);
+            c1 = scale_against(ref, kLog2e);
+        }
         o = ref * c;
         o1 = ref * c1;
-        inv = __fdividef(1.f, s);
-        inv1 = n.two ? __fdividef(1.f, s_hard) : inv;
+        // (a row without targets: its sums may be anything, and 0 / 0 is NaN)
+        const bool none = rec.A == 0.f && rec.B == 0.f;
+        inv = none ? 0.f : __fdividef(1.f, s);
+        inv1 = n.two && !none ? __fdividef(1.f, s_hard) : inv;
         ratio = 0.f;
         if (n.tail && n.soft && rec.has && s_out > 0.f) ratio = fmaxf(1.f - sq, 0.f) * __fdividef(s, s_out);
         soft_factors(n, rec, sq);
@@ -277,8 +283,6 @@ struct RowResult {
         }
     }
     __device__ __forceinline__ Gradient dense(const Needs& n, const Record& rec) const {
-        // a row without targets: its sums may be anything (0 inv is NaN for one of -inf)
-        if (rec.A == 0.f && rec.B == 0.f) return {0.f, 0.f, c, 0.f, c1, 0.f};
         if (!n.two) return {((n.soft ? rest : 0.f) + (n.hard ? rec.B : 0.f)) * inv, 0.f, c, o, c1, 0.f};  // one softmax
         if (rest != 0.f) return {rest * inv, rec.B * inv1, c, o, c1, o1};
         return {rec.B * inv1, 0.f, c1, o1, c1, 0.f};
@@ -540,7 +544,7 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
             auto add = [&](const uint4& raw) {
                 float v[EPV];
                 Chunk<T>::unpack(raw, v);
-                add_chunk<EPV>(x, v, need.two, need.c, o, kLog2e, o1);
+                add_chunk<EPV>(x, v, need, o, o1);
             };
             for (int p0 = 0; p0 < chunks; p0 += kSlot) {
                 stream_wait(full + sums_at.slot, sums_at.phase, ws);
@@ -763,7 +767,7 @@ distill_warp_kernel(const DistillArgs a, uint32_t rows)
             number = numbers.of(row + teams);
         }
         if (kSums) {
-            float ref = rec.ref, s_out, s_named, s_hard, soft = rec.soft, hard = rec.hard;
+            float ref = rec.ref, s_out, s_named, s_hard;
             if (marks) {
                 __syncwarp();
                 e.each([&](int, float&, float&, int&, int& pos) {
@@ -771,15 +775,13 @@ distill_warp_kernel(const DistillArgs a, uint32_t rows)
                 });
                 __syncwarp();
             }
-            for (int again = 0;; ++again) {
-                // (the first time with the offsets that the record's part was formed with)
-                const float c = again ? scale_against(ref, need.c) : need.c, c1 = again ? scale_against(ref, kLog2e) : kLog2e;
-                const float o = again ? ref * c : offset_against(ref, c), o1 = again ? ref * c1 : offset_against(ref, c1);
+            {
+                const float o = offset_against(ref, need.c), o1 = offset_against(ref, kLog2e);
                 Sums x{};
                 auto add = [&](const uint4& raw) {
                     float v[EPV];
                     Chunk<T>::unpack(raw, v);
-                    add_chunk<EPV>(x, v, need.two, c, o, c1, o1);
+                    add_chunk<EPV>(x, v, need, o, o1);
                 };
                 int p = 0;
                 for (; p + 32 * U <= chunks; p += 32 * U) {
@@ -791,25 +793,32 @@ distill_warp_kernel(const DistillArgs a, uint32_t rows)
                 }
 #pragma unroll 1
                 for (p += lane; p < chunks; p += 32) add(from[p - lane]);
-                join_sums(make_float4(x.soft, soft, x.hard + hard, 0.f), s_out, s_named, s_hard);
-                if (again || (sum_serves(s_out + s_named) && (!need.two || sum_serves(s_hard)))) break;
+                join_sums(make_float4(x.soft, rec.soft, x.hard + rec.hard, 0.f), s_out, s_named, s_hard);
+            }
+            if (!sum_serves(s_out + s_named) || (need.two && !sum_serves(s_hard))) {
                 // an overflow, or no reference of the row's: against the row's maximum
                 float m = -INFINITY;
+#pragma unroll 1
                 for (int i = lane; i < chunks * EPV; i += 32) m = fmaxf(m, to_float(l[i]));
                 e.each([&](int, float&, float& x, int&, int& pos) {
                     if (pos >= 0) m = fmaxf(m, x);
                 });
                 m = warp_max(m);
                 ref = m == -INFINITY ? 0.f : m;
-                soft = hard = 0.f;
-                if (marks) {
-                    const float c = scale_against(ref, need.c), c1 = scale_against(ref, kLog2e);
-                    e.each([&](int, float&, float& x, int&, int& pos) {
-                        if (pos < 0) return;
-                        soft += tc::exp2_approx(fmaf(x, c, -ref * c));
-                        if (need.two) hard += tc::exp2_approx(fmaf(x, c1, -ref * c1));
-                    });
+                const float c = scale_against(ref, need.c), c1 = scale_against(ref, kLog2e), o = ref * c, o1 = ref * c1;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                for (int i = lane; i < chunks * EPV; i += 32) {
+                    x.x += tc::exp2_approx(fmaf(to_float(l[i]), c, -o));
+                    if (need.two) x.z += tc::exp2_approx(fmaf(to_float(l[i]), c1, -o1));
                 }
+                if (marks)
+                    e.each([&](int, float&, float& t, int&, int& pos) {
+                        if (pos < 0) return;
+                        x.y += tc::exp2_approx(fmaf(t, c, -o));
+                        if (need.two) x.z += tc::exp2_approx(fmaf(t, c1, -o1));
+                    });
+                join_sums(x, s_out, s_named, s_hard);
             }
             const float sq = warp_reduce(rec.sq, SumOp()), kl = warp_reduce(rec.kl, SumOp());
             res.from_sums(need, rec, ref, s_out, s_named, s_hard, sq);
