@@ -3,7 +3,7 @@
 // Order: value descending, index ascending among equals; NaN after -inf.  With
 // keys whose ascending order is that of descending values, an entry is the
 // number key 2^32 + index and the record is the k smallest entries in order.
-// lse = ref/tau + log sum exp((l - ref)/tau).
+// lse = ref/tau + log sum exp((l - ref)/tau); a NaN makes it NaN, else a +inf +inf.
 // No row is sorted.  The k-th largest of the maxima of more than k groups of a row's
 // logits is a lower bound of its k-th largest logit, and a close one: the few
 // logits that reach it are collected and sorted.
@@ -211,7 +211,7 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
             for (int i = 0; i < kPerThread; ++i) s[i & 3] += tc::exp2_approx(fmaf(v[i], scale, -o));
             const float sum = warp_reduce((s[0] + s[1]) + (s[2] + s[3]), SumOp());
             if (lane == 0)
-                a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, scale, -o));
+                a.lse[row] = top == INFINITY && sum == sum ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, scale, -o));
         }
         float bound;  // at least k logits reach it, and not many more
         // (groups: twice as many as k that have a logit)
@@ -479,7 +479,7 @@ top_stream_kernel(const TopArgs a, uint32_t rows, const TopShape shape)
                         if (slices > 1) sum = warp_reduce(exchange(make_float4(sum, 0.f, 0.f, 0.f)).x, SumOp());
                     }
                     if (rank == 0 && lane == 0)
-                        a.lse[row] = top == INFINITY ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, scale, -o));
+                        a.lse[row] = top == INFINITY && sum == sum ? top : ref * inv_tau + (logf(sum) - kLn2 * fmaf(ref, scale, -o));
                 }
                 stream_wait(collected + b, phase, ws);
                 int n = counts[b];

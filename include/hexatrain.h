@@ -528,7 +528,8 @@ enum { HX_DTYPE_F32 = 0, HX_DTYPE_BF16 = 1, HX_DTYPE_F16 = 2 };
 /* The k largest logits of every row, value descending, the lowest index first
  * among equals (a NaN ranks after -inf): values[rows*k] in float32,
  * indices[rows*k], and, where lse is not NULL, lse[rows] = log sum_i
- * exp(l_i / temperature), the normaliser of the record's tail.  1 <= k <=
+ * exp(l_i / temperature), the normaliser of the record's tail (NaN where a logit
+ * is).  1 <= k <=
  * min(256, vocab); float32 rows of more than 262140 logits that are not 16-byte
  * aligned are served up to k = 224 (HX_ERR_UNSUPPORTED beyond). */
 int hx_top_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,

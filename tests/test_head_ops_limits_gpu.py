@@ -241,6 +241,21 @@ def test_rows_at_the_lowest_value(rt, torch, vocab, dtype, lowest):  # noqa: F81
             assert np.all(np.isfinite(d.backward()))
 
 
+# -- infinity and NaN in one row -----------------------------------------------------------
+
+@pytest.mark.parametrize("vocab", [50, 1024, 3000, 40000])
+def test_top_nan_beside_infinity(rt, torch, vocab):  # noqa: F811
+    """The largest logit is +inf, the log-sum-exp NaN: a NaN takes part in it."""
+    x = normal(3, 4, vocab)
+    x[0, 7] = x[1, 7] = np.inf
+    x[1, vocab - 1] = np.nan
+    x[2, 7] = np.nan
+    for dtype in ("f32", "bf16", "f16"):
+        v, i, s, _ = top(rt, torch, x, dtype, 3)
+        assert i[0, 0] == 7 and i[1, 0] == 7 and np.all(np.isfinite(v[:2, 1:]))
+        assert s[0] == np.inf and np.isnan(s[1]) and np.isnan(s[2]) and np.isfinite(s[3])
+
+
 # -- a reference far from the row's largest logit ---------------------------------------------
 
 @pytest.mark.parametrize("above", [60.0, 200.0])
