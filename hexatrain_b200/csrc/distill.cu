@@ -258,7 +258,11 @@ struct RowResult {
         inv = none ? 0.f : __fdividef(1.f, s);
         inv1 = n.two && !none ? __fdividef(1.f, s_hard) : inv;
         ratio = 0.f;
-        if (n.tail && n.soft && rec.has && s_out > 0.f) ratio = fmaxf(1.f - sq, 0.f) * __fdividef(s, s_out);
+        if (n.tail && n.soft && rec.has && s_out > 0.f) {
+            // (s / s_out overflows where s_out is near 2^-126: no mass either)
+            const float r = fmaxf(1.f - sq, 0.f) * __fdividef(s, s_out);
+            ratio = r < INFINITY ? r : 0.f;
+        }
         soft_factors(n, rec, sq);
     }
     // one lane writes the row's loss and statistics

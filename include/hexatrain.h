@@ -548,7 +548,8 @@ int hx_top_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t voca
  * A row without entries (or, renormalised, with none above -inf) has no KL
  * term; one whose label is negative, or every row when labels is NULL, has no
  * hard term; with neither, loss and gradient are 0.  Where the record leaves
- * the student no mass (p_T = 0) the tail bucket is left out.  The gradient is the
+ * the student no mass (p_T = 0, or too little for q_T / p_T in float32) the tail bucket
+ * is left out.  The gradient is the
  * derivative of that loss,
  *   dloss/dl_i = kd_weight tau (p_i c_i - q_i) + ce_weight (softmax(l)_i - [i = label]),
  * with c_i = S for the record's tokens and S - q_T / p_T for the others (S for all

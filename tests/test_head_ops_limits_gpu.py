@@ -256,6 +256,26 @@ def test_top_nan_beside_infinity(rt, torch, vocab):  # noqa: F811
         assert s[0] == np.inf and np.isnan(s[1]) and np.isnan(s[2]) and np.isfinite(s[3])
 
 
+# -- a tail at the edge of float32 ---------------------------------------------------------
+
+@pytest.mark.parametrize("vocab", [300, 1000, 1900, 9000, 40000])
+def test_distill_tail_at_the_edge_of_float32(rt, torch, vocab):  # noqa: F811
+    """200 equal named logits and one other token: its share is 2^-133 or 2^-132, below what
+    a float32 quotient holds, then 2^-114."""
+    k, tau, kd = 200, 1.0, 0.5
+    x = np.full((3, vocab), -np.inf, np.float32)
+    x[:, :k] = 0.0
+    x[:, k] = (-87.0, -86.5, -74.0)
+    rec = (np.zeros((3, k), np.float32), np.broadcast_to(np.arange(k, dtype=np.int32), (3, k)).copy(),
+           np.full(3, np.log(k) + 0.5, np.float32))
+    want, grad = soft64(x.astype(np.float64), rec, tau, kd)
+    d = Distill(rt, torch, x, "f32", rec, None, tau, kd, 0.0)
+    tol = 4 * (2 * REL + 8 * ULP * 100)
+    for g in ((d.forward(), d.backward())[1], d.fused()[1]):
+        assert np.all(np.abs(g - grad) <= tol * kd), np.abs(g - grad).max()
+    assert np.all(np.abs(d.fused()[0] - want) <= tol * kd * 4)
+
+
 # -- a reference far from the row's largest logit ---------------------------------------------
 
 @pytest.mark.parametrize("above", [60.0, 200.0])
