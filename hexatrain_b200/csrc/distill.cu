@@ -114,6 +114,8 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
     if (bad) label = -1;
     rec.label = label;
     rec.l_label = label >= 0 ? logit(label) : 0.f;
+    // (a teacher that masks the whole row has a log-sum-exp of -inf, and no entries)
+    const float lse_teacher = __shfl_sync(0xffffffffu, number, 1);
     float most = -INFINITY, ref = -INFINITY;
     e.each([&](int, float& t, float& l, int& idx, int& pos) {
         t = n.exact ? t * n.inv_tau : t / a.tau;
@@ -127,7 +129,7 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
             l = logit(idx);
             most = fmaxf(most, t);
             ref = fmaxf(ref, l);
-            has |= n.tail || t != -INFINITY;
+            has |= (n.tail ? lse_teacher : t) != -INFINITY;
             named |= idx == label;
             if (span.holds(idx)) pos = span.position(idx);
         }
@@ -141,7 +143,7 @@ __device__ __forceinline__ Record form_record(const DistillArgs& a, const Needs&
     rec.ref = fabsf(ref) < INFINITY ? ref : 0.f;
     float log_z;
     if (n.tail) {
-        log_z = __shfl_sync(0xffffffffu, number, 1);
+        log_z = lse_teacher;
     } else {
         most = warp_max(most);
         float z = 0.f;

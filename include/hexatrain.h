@@ -545,8 +545,8 @@ int hx_top_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t voca
  *   KL = sum_j q_j (log q_j - log p_{i_j}) [+ q_T (log q_T - log p_T)],
  *   loss[row] = kd_weight tau^2 KL + ce_weight (logsumexp(l) - l_label).
  * An entry with i_j < 0 is empty; the entries of one row name distinct tokens.
- * A row without entries (or, renormalised, with none above -inf) has no KL
- * term; one whose label is negative, or every row when labels is NULL, has no
+ * A row without entries (or, renormalised, with none above -inf, or with a
+ * teacher_lse of -inf) has no KL term; one whose label is negative, or every row when labels is NULL, has no
  * hard term; with neither, loss and gradient are 0.  Where the record leaves
  * the student no mass (p_T = 0, or too little for q_T / p_T in float32) the tail bucket
  * is left out.  The gradient is the

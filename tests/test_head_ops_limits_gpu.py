@@ -276,6 +276,32 @@ def test_distill_tail_at_the_edge_of_float32(rt, torch, vocab):  # noqa: F811
     assert np.all(np.abs(d.fused()[0] - want) <= tol * kd * 4)
 
 
+# -- a teacher's row without logits ----------------------------------------------------------
+
+@pytest.mark.parametrize("vocab", [50, 1000, 9000, 40000])
+def test_distill_teacher_row_of_masked_logits(rt, torch, vocab):  # noqa: F811
+    """The record of a row that the teacher masks as a whole: values and log-sum-exp -inf.
+    There is no KL term, in either form of the record."""
+    rows, k = 4, 6
+    x = normal(vocab, rows, vocab)
+    t = normal(8, rows, vocab)
+    t[0] = t[1] = -np.inf
+    v, i, s, _ = top(rt, torch, t, "f32", k, 2.0)
+    assert np.all(v[:2] == -np.inf) and np.all(s[:2] == -np.inf)
+    y = np.array([-1, 3, 5, -1], np.int32)
+    for tail in (False, True):
+        rec = (v.astype(np.float32), i, s.astype(np.float32) if tail else None)
+        empty = (rec[0], np.where(np.arange(rows)[:, None] < 2, -1, i).astype(np.int32), rec[2])
+        a = Distill(rt, torch, x, "f32", rec, y, 2.0, 0.5, 0.5)
+        b = Distill(rt, torch, x, "f32", empty, y, 2.0, 0.5, 0.5)
+        tol = 4 * (2 * REL + 8 * ULP * 40)  # (their exponentials are taken against other logits)
+        assert np.all(np.abs(a.forward()[0] - b.forward()[0]) <= tol * 4)
+        assert np.all(np.abs(a.backward() - b.backward()) <= tol)
+        (la, ga), (lb, gb) = a.fused(), b.fused()
+        assert np.all(np.abs(la - lb) <= tol * 4) and np.all(np.abs(ga - gb) <= tol)
+        assert la[0] == 0 and not ga[0].any() and np.all(np.isfinite(ga))
+
+
 # -- a reference far from the row's largest logit ---------------------------------------------
 
 @pytest.mark.parametrize("above", [60.0, 200.0])
