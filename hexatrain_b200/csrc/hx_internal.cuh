@@ -145,8 +145,9 @@ struct Profiler {
 // 11-14, the Muon kernel 16, the wait self-test
 // (hx_runtime_check_wait_timeout) 21, and the kernels over logit rows 32.
 constexpr int kWaitProbeCode = 21;
-// Error-word code of the kernels over logit rows: a teacher index or a label
-// that is not below the vocabulary size.
+// Error-word codes of the asynchronous calls over logit rows: a token id, or a teacher
+// index or a label, that is not below the vocabulary size.
+constexpr int kHeadTokenCode = 30;
 constexpr int kHeadIndexCode = 31;
 constexpr int kHeadWaitCode = 32;  // a bounded wait of theirs
 
@@ -221,6 +222,9 @@ struct hx_runtime {
         if (code) {
             hx::check_cuda(cudaMemsetAsync(err_flag.ptr, 0, sizeof(int), stream), "cudaMemsetAsync");
             hx::check_cuda(cudaStreamSynchronize(stream), "cudaStreamSynchronize");
+            if (code == hx::kHeadTokenCode)
+                hx::fail(HX_ERR_ARGUMENT, "INVALID_TINY_LM_TOKEN: token id >= vocabulary size; results of this call are "
+                                          "invalid");
             if (code == hx::kHeadIndexCode)
                 hx::fail(HX_ERR_ARGUMENT, "INVALID_DISTILL_INDEX: a teacher index or label is not below the vocabulary "
                                           "size; results of this call are invalid");

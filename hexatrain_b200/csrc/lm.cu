@@ -1314,7 +1314,7 @@ int hx_lm_train_step(hx_runtime* rt, const uint32_t* tokens, uint32_t step, floa
         lm_run(rt, p, lm_key(kGraphTrainStep, a.at<uint32_t>(p.tokens), gs), [&] {
             HX_CUDA(cudaMemsetAsync(a.at<int>(p.bad), 0, sizeof(int), rt->stream));
             ::hx::pdl_launch(split_tokens_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, rt->stream, 
-                p.B, p.T, p.V, a.at<uint32_t>(p.tokens), a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad));
+                p.B, p.T, p.V, a.at<uint32_t>(p.tokens), a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad), 1);
             HX_LAUNCHED(rt);
             forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), gs);
             optimizer_enqueue(rt, p);
@@ -1342,7 +1342,7 @@ int hx_lm_forward_backward_device(hx_runtime* rt, const uint32_t* tokens, float 
         const Arena& a = p.arena;
         lm_run(rt, p, lm_key(kGraphForwardBackward, tokens, grad_scale), [&] {
             ::hx::pdl_launch(split_tokens_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, rt->stream, 
-                p.B, p.T, p.V, tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad));
+                p.B, p.T, p.V, tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad), 1);
             HX_LAUNCHED(rt);
             forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), grad_scale);
         });
@@ -1356,9 +1356,10 @@ int hx_lm_top_logits_device(hx_runtime* rt, const uint32_t* tokens, uint32_t k, 
         require(tokens, HX_ERR_ARGUMENT, "top logits: null tokens");
         require(p.state_ready, HX_ERR_STATE, "top logits before state upload");
         const Arena& a = p.arena;
+        int* bad = rt->device_error();
         lm_run(rt, p, record_key(kGraphTopLogits, tokens, 0.f, values, indices, lse, k, temperature, 0.f, 0.f), [&] {
             ::hx::pdl_launch(split_tokens_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, rt->stream, p.B, p.T, p.V,
-                             tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad));
+                             tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), bad, kHeadTokenCode);
             HX_LAUNCHED(rt);
             forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), 1.0f, kForwardAllRows);
             head::top_logits(rt, HX_DTYPE_F32, uint32_t(p.M),
@@ -1377,11 +1378,12 @@ int hx_lm_distill_forward_backward_device(hx_runtime* rt, const uint32_t* tokens
         require(std::isfinite(grad_scale) && grad_scale > 0.f, HX_ERR_ARGUMENT, "forward_backward: invalid grad_scale");
         require(p.state_ready, HX_ERR_STATE, "forward_backward before state upload");
         const Arena& a = p.arena;
+        int* bad = rt->device_error();
         const SoftTargets soft{k, teacher_values, teacher_indices, teacher_lse, temperature, kd_weight, ce_weight};
         lm_run(rt, p, record_key(kGraphDistill, tokens, grad_scale, teacher_values, teacher_indices, teacher_lse, k,
                                  temperature, kd_weight, ce_weight), [&] {
             ::hx::pdl_launch(split_tokens_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, rt->stream, p.B, p.T, p.V,
-                             tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), a.at<int>(p.bad));
+                             tokens, a.at<int>(p.in_ids), a.at<int>(p.tgt_ids), bad, kHeadTokenCode);
             HX_LAUNCHED(rt);
             forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), grad_scale, kFullStep, &soft);
         });

@@ -28,14 +28,14 @@ __device__ __forceinline__ float warp_sumf(float v) {
 
 // tokens [B, T+1] -> input ids / target ids [B*T].  Any id >= V sets *bad.
 __global__ void split_tokens_kernel(int B, int T, int V, const uint32_t* __restrict__ tokens,
-                                    int* __restrict__ in_ids, int* __restrict__ tgt_ids, int* bad)
+                                    int* __restrict__ in_ids, int* __restrict__ tgt_ids, int* bad, int code)
 {
     HX_PDL_PROLOGUE();
     const int M = B * T;
     for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < M; r += gridDim.x * blockDim.x) {
         const int b = r / T, t = r % T;
         const uint32_t a = tokens[(size_t)b * (T + 1) + t], y = tokens[(size_t)b * (T + 1) + t + 1];
-        if (a >= (uint32_t)V || y >= (uint32_t)V) atomicExch(bad, 1);
+        if (a >= (uint32_t)V || y >= (uint32_t)V) atomicCAS(bad, 0, code);
         in_ids[r] = a < (uint32_t)V ? (int)a : 0;
         tgt_ids[r] = y < (uint32_t)V ? (int)y : 0;
     }

@@ -65,9 +65,12 @@ class Distiller:
         self._check(self.student.lm_optimizer_step_device(step), self.student)
 
     def loss(self) -> float:
-        """The mean loss of the last step (waits for it)."""
+        """The mean loss of the last step (waits for it).  Raises what either runtime
+        found wrong since the last time, a token id beyond the vocabulary among it."""
         p, n = self.student.lm_grad_buffer()
-        self._check(self.student.synchronize(), self.student)
+        done = [(rt.synchronize(), rt) for rt in (self.teacher, self.student)]
+        for ok, rt in done:
+            self._check(ok, rt)
         return float(_device_view(p, n)[-1])
 
 

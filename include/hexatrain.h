@@ -598,7 +598,9 @@ int hx_sample_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t v
 /* -- the same on the prepared LM ------------------------------------------ */
 /* A teacher's record: the forward of the device state on tokens [batch, T+1]
  * (device, as for hx_lm_forward_backward_device) and the top logits of every
- * position, values and indices [batch*T*k], lse [batch*T] (may be NULL). */
+ * position, values and indices [batch*T*k], lse [batch*T] (may be NULL).  Here and
+ * in the next call a token id not below the vocabulary counts as 0, and the next
+ * synchronising call fails with "INVALID_TINY_LM_TOKEN: ...". */
 int hx_lm_top_logits_device(hx_runtime* rt, const uint32_t* tokens, uint32_t k, float temperature, float* values,
                             int32_t* indices, float* lse);
 /* hx_lm_forward_backward_device with the distillation loss in place of the
