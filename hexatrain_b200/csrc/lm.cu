@@ -1179,11 +1179,10 @@ int hx_lm_generate_device(hx_runtime* rt, const uint32_t* prompts, uint32_t prom
                                   cudaMemcpyHostToDevice, s));
         HX_CUDA(cudaMemcpyAsync(d_uniform, numbers.data(), n * 4, cudaMemcpyHostToDevice, s));
         HX_CUDA(cudaMemcpyAsync(settings, set.data(), set.size() * 4, cudaMemcpyHostToDevice, s));
-        HX_CUDA(cudaMemsetAsync(a.at<int>(p.bad), 0, sizeof(int), s));
         for (uint32_t step = 0; step < max_new; ++step) {
             ::hx::pdl_launch(generation_window_kernel, grid_for(p.M, 256, rt->sm_count), 256, 0, s, int(B), int(T), int(room),
                              int(prompt_len + step), step ? d_tokens + size_t(step - 1) * B : nullptr, history,
-                             a.at<int>(p.in_ids), a.at<int>(p.bad));
+                             a.at<int>(p.in_ids));
             HX_LAUNCHED(rt);
             forward_backward(rt, p, a.at<float>(p.params), a.at<float>(p.grads), 1.0f, kForwardLastRow);
             head::sample_logits(rt, HX_DTYPE_F32, B,

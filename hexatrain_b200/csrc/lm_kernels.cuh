@@ -847,22 +847,18 @@ __global__ void widen_loss_kernel(int M, const float* __restrict__ loss, double*
 }
 
 // One step of generation on the device: appends the tokens of the step before (if
-// any; a token of -1 raises *bad and counts as 0) to the streams' histories
+// any; a token of -1 counts as 0) to the streams' histories
 // [B, room], and writes their windows, the last T of `length` tokens
 // right-aligned over 0 (buildTokenContext, nicopedia_byte_bpe.h:278-291).
 __global__ void generation_window_kernel(int B, int T, int room, int length, const int32_t* __restrict__ last,
-                                         uint32_t* history, int* __restrict__ ids, int* __restrict__ bad)
+                                         uint32_t* history, int* __restrict__ ids)
 {
     HX_PDL_PROLOGUE();
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < B * T; i += gridDim.x * blockDim.x) {
         const int b = i / T, at = length - T + i % T;
         int id = 0;
         if (last && at == length - 1) {
-            id = last[b];
-            if (id < 0) {
-                *bad = 1;
-                id = 0;
-            }
+            id = max(last[b], 0);
             history[size_t(b) * room + at] = uint32_t(id);
         } else if (at >= 0) {
             id = int(history[size_t(b) * room + at]);
