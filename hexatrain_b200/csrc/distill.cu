@@ -351,9 +351,10 @@ __device__ __forceinline__ void join_sums(float4 p, float& s_out, float& s_named
 // from memory once.  The exponentials are taken against the largest logit that
 // the record or the label names, known before the row's sums begin: no maximum
 // is looked for unless the sum overflows.
-// Measured: 4096x65536 bf16 fused at one temperature 198 us, 5.4 TB/s of 6.55 (at two
-// 290 us: four exponentials a logit fill the special-function unit for 236 us);
-// 16384x8192 float32 fused 172 us, 6.2 TB/s; 2048x32768 float16 backward 48 us.
+// Measured: 4096x65536 bf16 fused at one temperature 212 us, 5.1 TB/s of 6.55 (at two
+// 293 us: four exponentials a logit fill the special-function unit for 236 us; the loss
+// alone 144 us, two of them); 16384x8192 float32 fused 176 us, 6.1 TB/s, with a tail
+// 189; 2048x32768 float16 backward 48 us.
 struct StreamShape {
     int ring;        // slots
     int slices;      // CTAs of a row, a power of two
@@ -667,8 +668,8 @@ distill_stream_kernel(const DistillArgs a, uint32_t rows, const StreamShape shap
 // Rows of up to kChunks chunks (4 or 8 KB).  Each warp streams rows of its own
 // through two buffers in shared memory, the logits by cp.async.bulk and the record
 // by cp.async, so that the next row is in flight while one is worked on and no
-// barrier wider than the warp is met.  Measured: 131072x1024 float32 fused, k 32, 198 us,
-// 5.6 TB/s; one row per 128 threads with the row in registers took 287 us.
+// barrier wider than the warp is met.  Measured: 131072x1024 float32 fused, k 32, 196 us,
+// 5.7 TB/s; one row per 128 threads with the row in registers took 287 us.
 constexpr int kWarpRows = 2, kWarpTeams = 4;
 
 template <int kChunks>
@@ -933,6 +934,11 @@ void launch_warp(hx_runtime* rt, const DistillArgs& a, uint32_t rows)
     HX_LAUNCHED(rt);
 }
 
+// By the row's bytes: up to 8 KB a warp, 16 KB 128 consumers, 32 KB 256, then 512.  134 MB
+// of float32 logits, k 64, tail, loss + gradient in us, the other variant in brackets:
+// 7.6 KB 64 (109 by 128), 14 KB 76 (86 by 256), 19 KB 76 (94 by 128), 30 KB 62 (78 by
+// 512), 36 KB 76 (78 by 256).  For 16-bit rows of 19 and 36 KB, and for the loss or
+// the gradient alone, the smaller block would be 4 to 23 % faster there.
 template <class T, int kPass>
 void launch_distill(hx_runtime* rt, const DistillArgs& a, uint32_t rows)
 {

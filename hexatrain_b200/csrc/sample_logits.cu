@@ -70,7 +70,11 @@ constexpr float kNoMass = 24.f;               // tokens beyond have no mass: exp
 constexpr uint32_t kNoMassKey = 0x41c00000u;  // the bits of 24.0
 constexpr int kFine = 512;                    // buckets of a bucket's own histogram
 constexpr int kList = 256;                    // tokens that are collected and sorted at once
-constexpr int kFew = 224;                     // a top_k that is taken from one list
+// A top_k that is taken from one list: with it the tokens of the bucket in which it
+// ends have to fit.  Counting alone against masses for all, top_k 1, 50 and 200 for all
+// rows: 256x32768 float32 49, 55 and 74 us (62, 64, 66), 4096x4096 float16 58, 72 and 107
+// (82, 90, 92): better but for the widest.
+constexpr int kFew = 224;
 // Buckets of the row's histogram, equal steps of y: few tokens in each, and few
 // threads of a warp in the same.
 __host__ __device__ constexpr int coarse_buckets(int nt) { return nt == 128 ? 512 : 2048; }
@@ -271,10 +275,10 @@ __device__ __noinline__ uint64_t list_mass(const uint64_t* list, int c, float li
 // One block per row, or a cluster of them with a slice each, held in shared memory.
 // The first warp of the first CTA thinks, all others make the passes that it asks
 // for: the row's histogram, the collection of a bucket's tokens, rarely a bucket's
-// own histogram or the nth of equal tokens.  Bound by the instructions of the passes (about
-// 25 per token in the first, which forms expf of every one) and by the latency
+// own histogram or the nth of equal tokens.  Bound by the instructions of the passes (2 to 4
+// a token; the first forms expf of every one) and by the latency
 // between them: 256x32768 float32 57 us, 4096x4096 float16 74 us, one row of 1024
-// 10 us.  Few-token filters (top_k <= kFew) need no masses but those of
+// 7 to 12 us.  Few-token filters (top_k <= kFew) need no masses but those of
 // the tokens they keep: their histogram only counts.
 template <class T, int NT>
 __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8)

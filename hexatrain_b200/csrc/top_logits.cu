@@ -122,7 +122,7 @@ __device__ __noinline__ int exact_list(const T* row, int e0, int e1, float bound
 // ---- short rows: a warp per row ---------------------------------------------------
 // Rows of up to 1024 logits (with the lead): 32 to a lane, in registers, read from
 // the second of two buffers while the next row's copy is in flight.  Bound by the
-// instructions of the selection (about 1400 a row at k = 32): 131072x1024 float32 216 us, 2.6 TB/s.
+// instructions of the selection (about 1400 a row at k = 32): 131072x1024 float32 218 us, 2.6 TB/s.
 constexpr int kTopTeams = 4;
 // Entries that a warp's list holds.
 __host__ __device__ constexpr int top_list(int k) { return k <= 32 ? 128 : k <= 96 ? 256 : 512; }
@@ -304,7 +304,7 @@ top_warp_kernel(const TopArgs a, uint32_t rows)
 // finds the bound (in a cluster one for all CTAs), sorts what was collected, and one
 // CTA's warp, in turn, merges the CTAs' lists.  Bound
 // by instructions, two looks at every chunk and the row warps' sorts: 2048x131072
-// bfloat16, k 128, 276 us, 1.9 TB/s; 8192x16384 float32, k 64, 146 us, 3.7 TB/s.
+// bfloat16, k 128, 276 us, 1.9 TB/s; 8192x16384 float32, k 64, 145 us, 3.7 TB/s.
 struct TopPost {
     float o, bound;
 };
@@ -676,6 +676,10 @@ void launch_top_stream(hx_runtime* rt, const TopArgs& a, uint32_t rows, long chu
     HX_LAUNCHED(rt);
 }
 
+// By the row's bytes: a warp while its registers hold the row, up to 16 KB 128 consumers,
+// 32 KB 256, then 512.  134 MB of float32 logits, k 64, in us, the other variant in
+// brackets: 14 KB 145 (154 by 256), 19 KB 98 (221 by 128), 30 KB 92 (82 by 512; bfloat16
+// 86, 94), 36 KB 78 (127 by 256; bfloat16 88, 82).
 template <class T>
 void launch_top(hx_runtime* rt, const TopArgs& a, uint32_t rows)
 {
