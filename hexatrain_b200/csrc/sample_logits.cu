@@ -351,6 +351,7 @@ sample_kernel(const SampleArgs a, int slices, int log_slices)
         for (int r = 0; r < slices; ++r) m = fmaxf(m, s.maxima[r]);
         nan = m == INFINITY;
     }
+    m += 0.f;  // a maximum of -0 would give +0 a y of -0, whose bits are no key
     if (nan || m == -INFINITY) {
         if (tid == 0 && rank == 0) {
             a.tokens[row] = -1;

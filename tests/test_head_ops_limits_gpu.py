@@ -3,7 +3,7 @@ leave a kernel little room.  Tolerances as in test_head_ops_gpu.py."""
 import numpy as np
 import pytest
 
-from test_head_ops_gpu import (CODES, REL, ROUND, ULP, Distill, normal, record_of,  # noqa: F401
+from test_head_ops_gpu import (CODES, REL, ROUND, ULP, Distill, check_sample, normal, record_of,  # noqa: F401
                                check_distill, check_top, loss64, lse64, rt,
                                sample, some_labels, to_device, top, torch)
 
@@ -351,3 +351,21 @@ def test_sample_probabilities_of_the_kept_tokens(rt, torch):  # noqa: F811
         seen = np.bincount(tok, minlength=vocab)
         assert np.all(prob[seen > 0] > 0) and np.all(prob[seen == 0] <= 1.01 / n)
         assert np.all(np.abs(lp - np.log(prob[tok])) <= 1e-5)
+
+
+# -- sampling: the two zeros -------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,vocab", [(40, 2), (40, 7), (20, 300), (9, 1024), (9, 4100), (5, 40000), (300, 9001)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_sample_both_zeros_as_the_largest_logit(rt, torch, rows, vocab, dtype):  # noqa: F811
+    """-0 and +0 are one logit: tokens of either are equally likely, in the order of their
+    indices."""
+    rng = np.random.default_rng(rows + vocab)
+    x = -np.abs(normal(vocab, rows, vocab)) - np.float32(0.5)
+    zeros = rng.random(x.shape) < 0.4
+    zeros[:, vocab // 2] = True
+    zeros[::5] = True
+    x[zeros] = np.where(rng.random(x.shape) < 0.5, 0.0, -0.0)[zeros]
+    u = rng.random(rows).astype(np.float32)
+    for s in (dict(), dict(p=0.9), dict(k=17), dict(k=700, p=0.5), dict(mp=0.3), dict(t=0.3), dict(t=0.0)):
+        check_sample(rt, torch, x, dtype, u, **s)
