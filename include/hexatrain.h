@@ -528,10 +528,10 @@ enum { HX_DTYPE_F32 = 0, HX_DTYPE_BF16 = 1, HX_DTYPE_F16 = 2 };
 /* The k largest logits of every row, value descending, the lowest index first
  * among equals (a NaN ranks after -inf): values[rows*k] in float32,
  * indices[rows*k], and, where lse is not NULL, lse[rows] = log sum_i
- * exp(l_i / temperature), the normaliser of the record's tail (NaN where a logit
- * is).  1 <= k <=
- * min(256, vocab); float32 rows of more than 262140 logits that are not 16-byte
- * aligned are served up to k = 224 (HX_ERR_UNSUPPORTED beyond). */
+ * exp(l_i / temperature), the normaliser of the record's tail (NaN where a
+ * logit is).  1 <= k <= min(256, vocab); float32 rows of more than 262140
+ * logits that are not 16-byte aligned are served up to k = 224
+ * (HX_ERR_UNSUPPORTED beyond). */
 int hx_top_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,
                          size_t stride, uint32_t k, float temperature, float* values, int32_t* indices,
                          float* lse);
@@ -546,25 +546,26 @@ int hx_top_logits_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t voca
  *   loss[row] = kd_weight tau^2 KL + ce_weight (logsumexp(l) - l_label).
  * An entry with i_j < 0 is empty; the entries of one row name distinct tokens.
  * A row without entries (or, renormalised, with none above -inf, or with a
- * teacher_lse of -inf) has no KL term; one whose label is negative, or every row when labels is NULL, has no
- * hard term; with neither, loss and gradient are 0.  Where the record leaves
- * the student no mass (p_T = 0, or too little for q_T / p_T in float32) the tail bucket
- * is left out.  The gradient is the
- * derivative of that loss,
- *   dloss/dl_i = kd_weight tau (p_i c_i - q_i) + ce_weight (softmax(l)_i - [i = label]),
- * with c_i = S for the record's tokens and S - q_T / p_T for the others (S for all
- * without a bucket), S the sum of the q in the loss: 1, or sum_j q_j where the
- * bucket is left out or teacher_lse makes that 1 or more.  An index or label
- * not below vocab is skipped, and the next synchronising call fails with
+ * teacher_lse of -inf) has no KL term; one whose label is negative, or every
+ * row when labels is NULL, has no hard term; with neither, loss and gradient
+ * are 0, whatever the row's logits.  Where the record leaves the student no
+ * mass (p_T = 0, or too little for q_T / p_T in float32) the tail bucket is
+ * left out.  The gradient is the derivative of that loss,
+ *   dloss/dl_i = kd_weight tau (p_i c_i - q_i)
+ *              + ce_weight (softmax(l)_i - [i = label]),
+ * with c_i = S for the record's tokens and S - q_T / p_T for the others (S for
+ * all without a bucket), S the sum of the q in the loss: 1, or sum_j q_j where
+ * the bucket is left out or teacher_lse makes that 1 or more.  An index or
+ * label not below vocab is skipped, and the next synchronising call fails with
  * "INVALID_DISTILL_INDEX: ...".
  *
  * _forward writes loss[rows] and stats[rows*3] = (logsumexp(l/tau),
  * logsumexp(l), q_T/p_T), which _backward reads; _forward_backward does both in
- * one pass over the logits.  (Beyond 2^24 in size, as for a row masked as a whole by
- * a low value, a float32 logsumexp does not hold the number of the row's logits:
- * _backward takes p = 0 there.)  The gradient, in the type of the logits, is
- * grad_scale * grad_loss[row] (1 where grad_loss is NULL) * dloss/dl;
- * d_logits may be the logits themselves (with the same stride). */
+ * one pass over the logits.  (Beyond 2^24 in size, as for a row masked as a
+ * whole by a low value, a float32 logsumexp does not hold the number of the
+ * row's logits: _backward takes p = 0 there.)  The gradient, in the type of the
+ * logits, is grad_scale * grad_loss[row] (1 where grad_loss is NULL) *
+ * dloss/dl; d_logits may be the logits themselves (with the same stride). */
 int hx_distill_forward_device(hx_runtime* rt, int dtype, uint32_t rows, uint32_t vocab, const void* logits,
                               size_t stride, uint32_t k, const float* teacher_values,
                               const int32_t* teacher_indices, const float* teacher_lse, const int32_t* labels,

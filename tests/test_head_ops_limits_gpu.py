@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 # -- many rows to a block, wide records ----------------------------------------------
 
 @pytest.mark.parametrize("rows,vocab,k,pad", [(2500, 2100, 255, 0), (2500, 4096, 256, 0), (1500, 4093, 256, 3),
-                                              (40, 151936, 256, 0), (40, 140001, 213, 3), (30, 262144, 224, 1),
+                                              (40, 150000, 256, 0), (40, 140001, 213, 3), (30, 262144, 224, 1),
                                               (30, 262141, 5, 4)])
 def test_top_wide_records_of_many_rows(rt, torch, rows, vocab, k, pad):  # noqa: F811
     """Float32 rows whose lists leave a block two row warps or one, several rows to
